@@ -28,7 +28,8 @@ enum {
   MOE_ERR_UNSUPPORTED = -2, /* geometry with no compiled kernel            */
   MOE_ERR_HIP = -3,         /* the HIP runtime reported an error           */
   MOE_ERR_EXHAUSTED = -4,   /* slot pool exhausted (every slot pinned)     */
-  MOE_ERR_DEVICE = -5,      /* a kernel flagged an out-of-range slot ref   */
+  MOE_ERR_DEVICE = -5,      /* a kernel flagged an out-of-range slot ref, or
+                               an entry of a paged batch out of range        */
   MOE_ERR_TIMEOUT = -6      /* a kernel's bounded wait for another workgroup
                                gave up (moe_stack_decode with
                                MOE_STACK_ORDINARY whose grid was not resident
@@ -306,8 +307,113 @@ int moe_event_elapsed_ms(void *start, void *stop, float *ms);
 /* Read and clear the device error word set by the kernels, synchronising
  * `stream`.  Returns MOE_OK, MOE_ERR_TIMEOUT (a bounded cross-workgroup wait
  * gave up; the message also says if a slot ref was out of range) or
- * MOE_ERR_DEVICE (an out-of-range slot ref, whose contribution was zero). */
+ * MOE_ERR_DEVICE (an out-of-range slot ref, whose contribution was zero, or an
+ * entry of a moe_kv_view's arrays out of range, which was not followed). */
 int moe_check_device_error(void *stream);
+
+/* ------------------------------------------------------------------------
+ * Operators around the expert block: what a decoder layer runs before and
+ * beside the calls above.  They have no counterpart in the reference, whose
+ * engines take them from their model library.  16-bit tensors are bf16 or fp16
+ * (`dtype`); 8-bit ones are e4m3 codes (largest value 448).  Sums, statistics
+ * and scales are fp32.  T = 0 returns MOE_OK and does nothing.
+ */
+enum { MOE_DTYPE_BF16 = 0, MOE_DTYPE_F16 = 1, MOE_DTYPE_E4M3 = 2 };
+
+/*
+ * Root-mean-square norm behind the residual's addition, for T rows:
+ *   h = round(x + residual)  (x itself where residual is NULL), written to sum
+ *   y = h * rsqrt(mean(h^2) + eps) * weight
+ * y goes to `y` (dtype) or, with `q` instead, to e4m3: per row and block of 128
+ * columns, scales = max(largest |y|, 1e-30) / 448 and q = round(y / scale); a
+ * block with a value that is not finite is NaN throughout.  Exactly one of y
+ * and q is given, q with scales.  x, residual: rows of `width` at the given
+ * strides (elements); weight [width]; y, q, sum [T, width] contiguous, scales
+ * [T, ceil(width / 128)].  Any width up to 16384, any alignment of the elements.
+ * y or sum may be x or residual where those are contiguous too.
+ */
+int moe_add_rms_norm(const void *x, int64_t x_stride, const void *residual,
+                     int64_t residual_stride, const void *weight, int32_t dtype, int32_t T,
+                     int32_t width, float eps, void *y, uint8_t *q, float *scales, void *sum,
+                     void *stream);
+
+/*
+ * 8-bit product with a scale per block of 128:
+ *   y[t, n] = sum_b x_scales[t, b] w_scales[n / 128, b]
+ *             sum_{k in block b} x[t, k] w[n, k]  (+ bias[n])
+ * x: e4m3 [T, K] with x_scales [T, ceil(K / 128)] (x_dtype MOE_DTYPE_E4M3), or
+ * 16 bits, which the call first turns into codes and scales as moe_add_rms_norm
+ * does (x_scales NULL).  w: e4m3 [N, K], w_scales [ceil(N / 128),
+ * ceil(K / 128)]; bias and y [T, N] of out_dtype (16 bits).  K a multiple of 16;
+ * x and w (and x's row stride) 16-byte aligned; x_stride in elements.
+ * workspace: at least moe_linear_fp8_workspace() bytes, 256-byte aligned; it
+ * needs no zeroing.
+ */
+size_t moe_linear_fp8_workspace(int32_t T, int32_t K, int32_t N, int32_t x_dtype);
+int moe_linear_fp8(const void *x, int32_t x_dtype, int64_t x_stride, const float *x_scales,
+                   const uint8_t *w, const float *w_scales, const void *bias, int32_t T,
+                   int32_t K, int32_t N, int32_t out_dtype, void *y, void *workspace,
+                   size_t workspace_bytes, void *stream);
+
+/*
+ * A key/value cache in pages and the batch that uses it.  k, v: [n_pages,
+ * kv_heads, page_size, head_dim] of `dtype`; page_size a power of two in [16,
+ * 256].  Sequence s holds lens[s] tokens, the new ones included, token j in page
+ * table[s, j / page_size]; its new tokens are the batch's rows starts[s] to
+ * starts[s + 1], and row starts[s] + i is at position lens[s] - (starts[s + 1] -
+ * starts[s]) + i.  The arrays are on the device: entries out of range (pages,
+ * starts that descend or pass the batch's rows, lengths past the table or below
+ * the new tokens) are not followed, and raise the device error that
+ * moe_check_device_error reports as MOE_ERR_DEVICE.  Rows behind the last
+ * sequence are left as they were in every output.
+ */
+typedef struct moe_kv_view {
+  void *k;
+  void *v;
+  const int32_t *table;    /* [n_seqs, table_width] */
+  const int32_t *starts;   /* [n_seqs + 1]          */
+  const int32_t *lens;     /* [n_seqs]              */
+  int32_t n_pages, kv_heads, page_size, head_dim, dtype;
+  int32_t n_seqs, table_width;
+} moe_kv_view;
+
+/*
+ * Rotary positions of T new tokens, and their keys and values into the cache:
+ *   q_out[t, h] = turn(norm(q[t, h])), page of k <- turn(norm(k)), of v <- v
+ * where turn takes pair i of the first `rot` dims, (i, i + rot/2) or with
+ * `interleaved` (2i, 2i + 1), by position * freqs[i] radians and times mscale,
+ * and norm is the root-mean-square norm of the head with q_weight / k_weight
+ * [head_dim] (NULL: none).  q [T, heads, head_dim], k and v [T, kv_heads,
+ * head_dim] at the given token and head strides (elements, the last dim
+ * contiguous); freqs [rot/2] fp64 on the device; q_out [T, heads, head_dim]
+ * contiguous, and it may be q.  head_dim even, up to 512.  Angles are reduced in
+ * fp64.
+ */
+int moe_rope_cache(const moe_kv_view *kv, const void *q, int64_t q_token, int64_t q_head,
+                   const void *k, int64_t k_token, int64_t k_head, const void *v,
+                   int64_t v_token, int64_t v_head, int32_t T, int32_t heads,
+                   const double *freqs, int32_t rot, int32_t interleaved, float mscale,
+                   const void *q_weight, const void *k_weight, float eps, void *q_out,
+                   void *stream);
+
+/*
+ * Attention of T new tokens over the cache (which holds their own keys and
+ * values already):
+ *   out[t, h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q[t, h] . k_j)
+ * over the keys j up to the row's own position, or the last `window` of those
+ * (window > 0).  Head h reads key head h / (heads / kv_heads).  sinks [heads]
+ * fp32 (NULL: none) adds exp(sinks[h]) to the sum below the line.  Keys that a
+ * row does not see, and what pages hold past a sequence's length, have no
+ * influence whatever their bits.  A row that sees no key is zero.  q at token
+ * and head strides that are multiples of 8 elements, 16-byte aligned; out [T,
+ * heads, head_dim] contiguous.  head_dim 64 or 128, up to 64 heads per key head.
+ * workspace: at least moe_attn_paged_workspace() bytes, 256-byte aligned; it
+ * needs no zeroing.
+ */
+size_t moe_attn_paged_workspace(const moe_kv_view *kv, int32_t T, int32_t heads);
+int moe_attn_paged(const moe_kv_view *kv, const void *q, int64_t q_token, int64_t q_head,
+                   int32_t T, int32_t heads, float scale, int32_t window, const float *sinks,
+                   void *out, void *workspace, size_t workspace_bytes, void *stream);
 
 /*
  * Slot-pool bookkeeping (host only, no device calls): the (layer, expert) ->

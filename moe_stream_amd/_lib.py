@@ -28,6 +28,9 @@ MOE_ACT_SWIGLU = 0
 MOE_ACT_SWIGLU_CLAMP = 1
 MOE_ROUTE_SOFTMAX_TOPK = 0
 MOE_ROUTE_TOPK_SOFTMAX = 1
+MOE_DTYPE_BF16 = 0
+MOE_DTYPE_F16 = 1
+MOE_DTYPE_E4M3 = 2
 MAX_COMPONENTS = 12
 MAX_TOPK = 16
 
@@ -40,6 +43,8 @@ EXPORTS = (
     "moe_ffn_grouped_workspace", "moe_ffn_grouped",
     "moe_route_workspace", "moe_route", "moe_slot_lookup",
     "moe_stack_workspace", "moe_stack_decode", "moe_stack_trace",
+    "moe_add_rms_norm", "moe_linear_fp8_workspace", "moe_linear_fp8",
+    "moe_rope_cache", "moe_attn_paged_workspace", "moe_attn_paged",
     "moe_fill_slots", "moe_host_alloc", "moe_host_free",
     "moe_event_create", "moe_event_destroy", "moe_event_record",
     "moe_event_query", "moe_stream_wait_event", "moe_event_elapsed_ms",
@@ -78,6 +83,14 @@ class PoolView(C.Structure):
                 ("comp_offset", C.c_int64 * MAX_COMPONENTS)]
 
 
+class KvView(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("table", C.c_void_p),
+                ("starts", C.c_void_p), ("lens", C.c_void_p),
+                ("n_pages", C.c_int32), ("kv_heads", C.c_int32), ("page_size", C.c_int32),
+                ("head_dim", C.c_int32), ("dtype", C.c_int32),
+                ("n_seqs", C.c_int32), ("table_width", C.c_int32)]
+
+
 _lib = None
 
 
@@ -109,6 +122,14 @@ def _declare(lib):
         "moe_stack_decode": (C.c_int, [C.POINTER(PoolView), C.POINTER(Geom), I32, I32, I32,
                                        P, P, P, I32, I32, I32, P, P, P, P, P, P, P,
                                        C.c_uint32, I32, P, SZ, P]),
+        "moe_add_rms_norm": (C.c_int, [P, I64, P, I64, P, I32, I32, I32, F, P, P, P, P, P]),
+        "moe_linear_fp8_workspace": (SZ, [I32, I32, I32, I32]),
+        "moe_linear_fp8": (C.c_int, [P, I32, I64, P, P, P, P, I32, I32, I32, I32, P, P, SZ, P]),
+        "moe_rope_cache": (C.c_int, [C.POINTER(KvView), P, I64, I64, P, I64, I64, P, I64, I64,
+                                     I32, I32, P, I32, I32, F, P, P, F, P, P]),
+        "moe_attn_paged_workspace": (SZ, [C.POINTER(KvView), I32, I32]),
+        "moe_attn_paged": (C.c_int, [C.POINTER(KvView), P, I64, I64, I32, I32, F, I32, P, P, P,
+                                     SZ, P]),
         "moe_fill_slots": (C.c_int, [C.POINTER(PoolView), P, I64, I64, P, P, I32, P]),
         "moe_host_alloc": (C.c_int, [SZ, C.POINTER(C.c_void_p)]),
         "moe_host_free": (C.c_int, [P]),

@@ -790,7 +790,12 @@ int moe_check_device_error(void *stream) {
                   "at once: another kernel held CUs of the device)%s",
                   (v & moe::kErrBadRef) ? "; a kernel also resolved an out-of-range slot "
                                           "reference" : "");
-    return fail(MOE_ERR_DEVICE, "a kernel resolved an out-of-range slot reference");
+    if (!(v & moe::kErrBadRef))
+      return fail(MOE_ERR_DEVICE, "a kernel met a page, a row start or a length of a paged "
+                  "batch outside its range");
+    return fail(MOE_ERR_DEVICE, "a kernel resolved an out-of-range slot reference%s",
+                (v & moe::kErrBadBatch) ? "; a kernel also met a page, a row start or a length "
+                                          "of a paged batch outside its range" : "");
   }
   return MOE_OK;
 }

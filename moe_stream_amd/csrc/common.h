@@ -260,6 +260,7 @@ __device__ __forceinline__ const char *resolve_packed_safe(const PoolArgs &pa, i
 // Bits of the device error word.
 constexpr int kErrBadRef = 1;    // a slot reference outside the pool view
 constexpr int kErrTimeout = 2;   // a bounded cross-workgroup wait gave up
+constexpr int kErrBadBatch = 4;  // a paged batch's page, row start or length out of range
 
 __device__ __forceinline__ void flag_error_bits(int bits) {
   __hip_atomic_fetch_or(&g_device_error, bits, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);

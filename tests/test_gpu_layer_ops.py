@@ -1,0 +1,527 @@
+"""The operators around the expert block on the GPU against 64-bit restatements of
+their definitions (oracle/layer.py).
+
+Bounds, with u = half a step of the output's type (2^-8 bf16, 2^-11 fp16):
+  norm    a row's sum of squares in 32 bits is off by at most 72 roundings of 2^-24
+          (64 products of a lane and 8 levels of lanes and waves), its root by half of
+          that, plus 4 for the quotient, root and products: under 2^-18 of the value,
+          and u for the store.
+  codes   half a step of e4m3 (2^-4 of the value, 2^-10 in its subnormal range), at the
+          scale, on top of the norm's 2^-18.
+  rope    a turn's fraction is rounded to 2^-25, an angle of 2^-22 radians; cosine, sine
+          and the two products add less than 2^-21 of |a| + |b|; with the heads' norm
+          2^-18 of it in all.
+  attn    a weight is rounded to the type's u of itself before the product with v, and
+          the score's 32-bit sum and the exponential are off by under 2^-14 of it here
+          (|q||k| scale below 2^6, 128 terms): (u + 2^-14) sum p|v| / sum p, and u for
+          the store.
+  linear  K + blocks roundings of 2^-23 (the matrix unit may truncate) of the sum of
+          magnitudes, and u for the store.
+"""
+import numpy as np
+import pytest
+import torch
+
+from moe_stream_amd import _lib, ops
+from moe_stream_amd import geometry as G
+from oracle import layer as O
+
+from helpers import Layer
+from layer_helpers import BF16, F16, F8, HALF, TINY, Batch, f64, randn, within
+
+pytestmark = pytest.mark.gpu
+
+
+# -- norm ---------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("T,D", [(1, 2048), (3, 2880), (1, 1), (5, 7), (2, 127), (4, 129),
+                                 (1025, 512), (1100, 2880), (1030, 1001), (2, 4097), (3, 8192),
+                                 (2, 16384), (1024, 4096), (1027, 65)])
+def test_norm_16_bits(T, D, dtype):
+    x, r = randn((T, D), 11, dtype, 0.7), randn((T, D), 12, dtype, 3.0)
+    w = randn((D,), 13, dtype)
+    y, h = ops.add_rms_norm(x, w, residual=r, eps=1e-5)
+    href = (x.double() + r.double()).to(dtype)
+    assert torch.equal(h, href)
+    ref = O.rms_norm(f64(href), f64(w), 1e-5)
+    within(y, ref, np.abs(ref) * (HALF[dtype] + 2.0 ** -18) + TINY[dtype])
+    y0, h0 = ops.add_rms_norm(h, w, eps=1e-5)
+    assert torch.equal(y0, y) and torch.equal(h0, h)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("T,D", [(1, 2048), (3, 2880), (2, 5), (3, 130), (1100, 2880), (1029, 333),
+                                 (2, 6001), (1030, 4096)])
+def test_norm_8_bits(T, D, dtype):
+    x, r, w = randn((T, D), 21, dtype), randn((T, D), 22, dtype), randn((D,), 23, dtype)
+    q, s, h = ops.add_rms_norm(x, w, residual=r, fp8=True)
+    href = (x.double() + r.double()).to(dtype)
+    assert torch.equal(h, href) and q.dtype == F8
+    ref = O.rms_norm(f64(href), f64(w), 1e-6)
+    _, sref = O.quant(ref)
+    within(s, sref, sref * 2.0 ** -17)
+    sc = np.repeat(sref, 128, 1)[:, :D]
+    got = f64(q) * np.repeat(f64(s), 128, 1)[:, :D]
+    bound = np.maximum(np.abs(ref) * 2.0 ** -4, sc * 2.0 ** -10) + np.abs(ref) * 2.0 ** -16
+    assert (np.abs(got - ref) <= bound).all()
+    # each block's largest value stands at the code's largest
+    top = np.abs(np.pad(f64(q), ((0, 0), (0, -D % 128)))).reshape(T, -1, 128).max(2)
+    assert (top == 448.0).all()
+
+
+def test_norm_takes_strided_rows_and_writes_in_place():
+    big = randn((9, 3000), 31)
+    x, r, w = big[:, 5:1505], randn((9, 1500), 32), randn((1500,), 33)
+    y, h = ops.add_rms_norm(x, w, residual=r)
+    yc, hc = ops.add_rms_norm(x.contiguous(), w, residual=r)
+    assert torch.equal(y, yc) and torch.equal(h, hc)
+    xi, ri = x.contiguous(), r.clone()
+    y2, h2 = ops.add_rms_norm(xi, w, residual=ri, out=xi, summed=ri)
+    assert y2 is xi and h2 is ri and torch.equal(xi, y) and torch.equal(ri, h)
+
+
+def test_norm_of_one_row_without_a_batch_and_of_none():
+    x, w = randn((2048,), 34), randn((2048,), 35)
+    y, h = ops.add_rms_norm(x, w)
+    assert y.shape == (2048,) and torch.equal(y, ops.add_rms_norm(x[None], w)[0][0])
+    y, h = ops.add_rms_norm(x[None][:0], w)
+    assert y.shape == (0, 2048)
+
+
+def test_norm_zero_rows_and_values_that_are_not_finite():
+    x = torch.zeros((4, 256), dtype=BF16, device="cuda")
+    x[1, 3], x[2, 200] = float("nan"), float("inf")
+    x[3] = 1.0
+    w = torch.ones(256, dtype=BF16, device="cuda")
+    q, s, _ = ops.add_rms_norm(x, w, fp8=True)
+    qf, sf = q.float().cpu(), s.cpu()
+    assert (qf[0] == 0).all() and torch.allclose(sf[0], torch.tensor(1e-30 / 448), rtol=1e-6)
+    assert qf[1].isnan().all()                 # the row's norm is NaN
+    assert qf[2, 128:].isnan().all()           # inf / inf; the other block is zero
+    assert (qf[2, :128] == 0).all()
+    assert (qf[3] == 448).all()
+
+
+# -- 8-bit product ----------------------------------------------------------------
+def _weights(N, K, seed):
+    w = randn((N, K), seed, torch.float32, 100.0).clamp(-448, 448).to(F8)
+    ws = randn((-(-N // 128), -(-K // 128)), seed + 1, torch.float32).abs() * 1e-3 + 1e-4
+    return w, ws
+
+
+LINEAR = [(1, 2048, 5120), (1, 16, 1), (2, 144, 130), (7, 2880, 257), (16, 4096, 640),
+          (17, 272, 2880), (33, 2048, 512), (64, 128, 96), (65, 1040, 1000), (128, 2048, 256),
+          (129, 400, 384), (255, 128, 129), (300, 2880, 520), (1000, 144, 100),
+          (2049, 256, 260), (515, 2048, 5120)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("T,K,N", LINEAR)
+def test_linear(T, K, N, dtype):
+    w, ws = _weights(N, K, 41)
+    x16 = randn((T, K), 43, dtype)
+    bias = randn((N,), 44, dtype)
+    xq, xs = O.quant(f64(x16))
+    ref, mag = O.linear(xq, xs, f64(w), f64(ws))
+    bound = mag * (K + 40) * 2.0 ** -23
+    y = ops.linear_fp8(x16, w, ws)
+    assert y.dtype == dtype
+    within(y, ref, np.abs(ref) * HALF[dtype] + bound + TINY[dtype])
+    # the same codes and scales given
+    q = torch.tensor(xq, device="cuda").to(F8)
+    s = torch.tensor(xs, device="cuda").float()
+    assert (f64(q) == xq).all()
+    y8 = ops.linear_fp8(q, w, ws, x_scales=s, dtype=dtype)
+    assert torch.equal(y8, y)
+    yb = ops.linear_fp8(q, w, ws, x_scales=s, dtype=dtype, bias=bias)
+    rb = ref + f64(bias)
+    within(yb, rb, np.abs(rb) * HALF[dtype] + bound + np.abs(rb) * 2.0 ** -22 + TINY[dtype])
+
+
+def test_linear_rows_do_not_depend_on_each_other():
+    """A row alone, among others, and of a strided x gives the same bits where the same
+    kernel runs, and a NaN row stays its own."""
+    w, ws = _weights(640, 1024, 51)
+    x = randn((200, 1024), 53)
+    y = ops.linear_fp8(x, w, ws)
+    x2 = x.clone()
+    x2[7, 100] = float("nan")
+    x2[150, 3] = float("inf")
+    y2 = ops.linear_fp8(x2, w, ws)
+    keep = [i for i in range(200) if i not in (7, 150)]
+    assert torch.equal(y2[keep], y[keep])
+    assert y2[7].isnan().all() and y2[150].isnan().all()
+    wide = torch.zeros((200, 2048), dtype=BF16, device="cuda")
+    wide[:, 512:1536] = x
+    assert torch.equal(ops.linear_fp8(wide[:, 512:1536], w, ws), y)
+
+
+def test_linear_of_one_row_without_a_batch_and_of_none():
+    w, ws = _weights(130, 256, 55)
+    x = randn((256,), 57)
+    y = ops.linear_fp8(x, w, ws)
+    assert y.shape == (130,) and torch.equal(y, ops.linear_fp8(x[None], w, ws)[0])
+    assert ops.linear_fp8(x[None][:0], w, ws).shape == (0, 130)
+
+
+# -- rotary positions ---------------------------------------------------------------
+ROPE = [dict(seqs=[(1, 1)], H=4, HK=1, D=64, R=64, page=16),
+        dict(seqs=[(1, 40000), (1, 17), (1, 129)], H=32, HK=4, D=128, R=128, page=64, norm=True),
+        dict(seqs=[(5, 5), (0, 30), (17, 40), (1, 16), (0, 0), (33, 100)], H=7, HK=1, D=64, R=20,
+             page=16, inter=True),
+        dict(seqs=[(700, 900), (400, 400)], H=8, HK=2, D=64, R=32, page=32, norm=True, inter=True),
+        dict(seqs=[(1200, 1200)], H=6, HK=2, D=80, R=80, page=128),
+        dict(seqs=[(3, 2 ** 20), (2, 77)], H=4, HK=4, D=128, R=64, page=256, norm=True),
+        dict(seqs=[(9, 11)], H=3, HK=3, D=10, R=6, page=16, norm=True),
+        dict(seqs=[(2, 33)], H=2, HK=1, D=512, R=512, page=16),
+        dict(seqs=[(4, 9)], H=2, HK=2, D=64, R=0, page=16, norm=True)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("c", ROPE, ids=lambda c: f"{len(c['seqs'])}x{c['D']}r{c['R']}")
+def test_rope_cache(c, dtype):
+    H, HK, D, R = c["H"], c["HK"], c["D"], c["R"]
+    b = Batch(c["seqs"], H, HK, D, c["page"], dtype, seed=61, extra_rows=2)
+    qkv = randn((b.T, H + 2 * HK, D), 65, dtype)
+    q, k, v = qkv[:, :H], qkv[:, H:H + HK], qkv[:, H + HK:]
+    qw = randn((D,), 66, dtype) if c.get("norm") else None
+    kw = randn((D,), 67, dtype) if c.get("norm") else None
+    freqs = torch.tensor(150000.0 ** (-np.arange(R // 2) / max(R // 2, 1)), device="cuda")
+    m = 1.25
+    kp0, vp0 = b.kp.clone(), b.vp.clone()
+    out = torch.full_like(b.q, 7.0)
+    got = ops.rope_cache(q, k, v, *b.pages(), freqs, interleaved=c.get("inter", False), mscale=m,
+                         q_weight=qw, k_weight=kw, eps=1e-5, out=out)
+    ops.check_device_error()
+    assert got is out
+    assert (out[b.rows:] == 7.0).all()                   # behind the last sequence
+    kref, vref = f64(kp0), f64(vp0)
+    kbound = np.zeros_like(kref)
+    for s in range(len(c["seqs"])):
+        rows, pos = b.span(s)
+        if not len(pos):
+            continue
+
+        def one(x, w):
+            x = f64(x[rows])
+            if w is not None:
+                x = O.rms_norm(x, f64(w), 1e-5)
+            y = O.turn(x, pos, f64(freqs), m, c.get("inter", False))
+            i = np.arange(R // 2)
+            mate = np.arange(D)
+            i0, i1 = (2 * i, 2 * i + 1) if c.get("inter") else (i, i + R // 2)
+            mate[i0], mate[i1] = i1, i0
+            a = np.abs(x) + np.abs(x[..., mate])
+            return y, np.abs(y) * HALF[dtype] + 2.0 ** -18 * m * a + TINY[dtype]
+
+        y, bound = one(q, qw)
+        within(out[rows], y, bound)
+        yk, bk = one(k, kw)
+        pg = b.np_table[s, pos // b.page]
+        kref[pg, :, pos % b.page], kbound[pg, :, pos % b.page] = yk, bk
+        vref[pg, :, pos % b.page] = f64(v[rows])
+    within(b.kp, kref, kbound + 1e-300)
+    assert (f64(b.vp) == vref).all()
+    # in place
+    qc = q.contiguous()
+    assert torch.equal(ops.rope_cache(qc, k, v, *b.pages(), freqs,
+                                      interleaved=c.get("inter", False), mscale=m, q_weight=qw,
+                                      k_weight=kw, eps=1e-5, out=qc)[:b.rows], out[:b.rows])
+
+
+def test_values_keep_their_bits():
+    """Values pass as bits, NaN payloads among them."""
+    b = Batch([(3, 3)], 2, 2, 64)
+    v = torch.arange(0x7f80, 0x7f80 + 3 * 128, dtype=torch.int32).to(torch.int16)
+    v = v.view(3, 2, 64).cuda().view(BF16)
+    f = torch.zeros(32, dtype=torch.float64, device="cuda")
+    ops.rope_cache(b.q, b.q, v, *b.pages(), f)
+    got = torch.stack([b.vp[b.np_table[0, 0], :, i] for i in range(3)])
+    assert torch.equal(got.view(torch.int16), v.view(torch.int16))
+
+
+# -- attention -----------------------------------------------------------------------
+ATTN = [dict(seqs=[(1, 1)], H=8, HK=1, D=128, page=16),
+        dict(seqs=[(1, 2500)], H=32, HK=4, D=128, page=64),
+        dict(seqs=[(1, 700), (1, 1), (1, 63), (1, 64), (1, 65), (1, 999)], H=64, HK=8, D=64,
+             page=16, sinks=True),
+        dict(seqs=[(3, 200), (1, 130), (5, 5), (2, 128), (4, 300)], H=16, HK=2, D=64, page=32,
+             window=128, sinks=True),
+        dict(seqs=[(5, 5), (0, 30), (17, 40), (1, 16), (0, 0), (33, 100)], H=7, HK=1, D=64,
+             page=16),
+        dict(seqs=[(150, 390), (70, 70)], H=12, HK=2, D=128, page=128, sinks=True),
+        dict(seqs=[(130, 200)], H=4, HK=4, D=64, page=16, window=1),
+        dict(seqs=[(257, 300), (31, 500)], H=10, HK=2, D=128, page=32, window=70),
+        dict(seqs=[(9, 400)], H=64, HK=1, D=64, page=256),
+        dict(seqs=[(40, 41), (2, 9)], H=66, HK=2, D=64, page=16, sinks=True),
+        dict(seqs=[(100, 600)], H=3, HK=1, D=128, page=16, window=33)]
+
+
+def _attn_ref(b, q, window, sinks, scale):
+    n, _, D = q.shape
+    ref, mag = np.zeros(q.shape), np.zeros(q.shape)
+    for s in range(len(b.seqs)):
+        rows, pos = b.span(s)
+        if len(pos):
+            ref[rows], mag[rows] = O.attention(f64(q[rows]), b.cached(s, b.kp), b.cached(s, b.vp),
+                                               pos, scale, window, sinks)
+    return ref, mag
+
+
+def _attn_bound(ref, mag, dtype):
+    return np.abs(ref) * HALF[dtype] + (HALF[dtype] + 2.0 ** -14) * mag + TINY[dtype]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("c", ATTN, ids=lambda c: f"{len(c['seqs'])}x{c['H']}h{c['HK']}d{c['D']}")
+def test_attn(c, dtype):
+    H, D, window = c["H"], c["D"], c.get("window", 0)
+    b = Batch(c["seqs"], H, c["HK"], D, c["page"], dtype, seed=71, fill=float("nan"),
+              extra_rows=3)
+    sinks = randn((H,), 72, torch.float32) if c.get("sinks") else None
+    out = torch.full_like(b.q, 7.0)
+    got = ops.attn_paged(b.q, *b.pages(), window=window, sinks=sinks, out=out)
+    ops.check_device_error()
+    assert got is out and (out[b.rows:] == 7.0).all()
+    ref, mag = _attn_ref(b, b.q[:b.rows], window, None if sinks is None else f64(sinks),
+                         D ** -0.5)
+    within(out[:b.rows], ref, _attn_bound(ref, mag, dtype))
+
+
+@pytest.mark.parametrize("D,H,HK,seqs", [(64, 8, 1, [(1, 5000), (1, 40), (1, 2100)]),
+                                         (128, 8, 2, [(40, 5000), (3, 1000)]),
+                                         (64, 16, 2, [(200, 2000)])])
+def test_attn_scores_far_apart(D, H, HK, seqs):
+    """One key takes nearly the whole weight, wherever it stands: the running maximum
+    moves late, and nothing overflows."""
+    b = Batch(seqs, H, HK, D, 32, BF16, seed=81)
+    for s, (n, L) in enumerate(seqs):
+        for j in (0, L // 2, L - n):
+            b.kp[b.np_table[s, j // 32], :, j % 32] *= 30.0
+    got = ops.attn_paged(b.q, *b.pages())
+    ref, mag = _attn_ref(b, b.q, 0, None, D ** -0.5)
+    # scores of up to 2^9: their 32-bit sums are off by up to 2^-12
+    bound = np.abs(ref) * 2.0 ** -8 + (2.0 ** -8 + 2.0 ** -10) * mag
+    within(got, ref, bound)
+
+
+@pytest.mark.parametrize("n", [1, 4, 40, 200])
+def test_attn_keys_that_a_row_does_not_see_have_no_influence(n):
+    """NaN and infinity in later tokens of the same chunk and in keys behind the
+    window: rows that do not see them keep their bits."""
+    L, window = 400, 90
+    b = Batch([(n, L), (2, 70)], 16, 2, 64, 16, BF16, seed=91)
+    base = ops.attn_paged(b.q, *b.pages(), window=window)
+    bad = {0: L - n - window - 5, 1: L - 1}            # behind every window; the last token
+    for i, j in bad.items():
+        pg = int(b.np_table[0, j // 16])
+        b.kp[pg, :, j % 16], b.vp[pg, :, j % 16] = float("inf"), float("nan")
+        b.vp[pg, :, j % 16, ::2] = float("-inf")
+    got = ops.attn_paged(b.q, *b.pages(), window=window)
+    assert torch.equal(got[:n - 1], base[:n - 1])       # all but the row that sees it
+    assert torch.equal(got[n:], base[n:])               # the other sequence
+    assert got[n - 1].isnan().any()
+
+
+def test_attn_rows_that_see_nothing():
+    """Rows before the sequence's first position (a length below the new tokens) are
+    zero, and reported."""
+    b = Batch([(6, 6), (3, 50)], 8, 1, 64)
+    b.lens[0] = 2
+    sinks = randn((8,), 95, torch.float32)
+    for s in (None, sinks):
+        out = ops.attn_paged(b.q, *b.pages(), sinks=s)
+        assert (out[:4] == 0).all() and (out[4:] != 0).any(-1).all()
+        with pytest.raises(_lib.MoeError) as e:
+            ops.check_device_error()
+        assert e.value.code == _lib.MOE_ERR_DEVICE
+
+
+def test_attn_sink_of_minus_infinity_is_none():
+    b = Batch([(4, 100)], 8, 1, 64)
+    s = torch.full((8,), float("-inf"), device="cuda")
+    assert torch.equal(ops.attn_paged(b.q, *b.pages(), sinks=s), ops.attn_paged(b.q, *b.pages()))
+
+
+def test_attn_strided_queries():
+    b = Batch([(30, 100), (1, 900)], 8, 2, 64)
+    wide = torch.zeros((b.T, 12, 64), dtype=BF16, device="cuda")
+    wide[:, 2:10] = b.q
+    want = ops.attn_paged(b.q, *b.pages())
+    assert torch.equal(ops.attn_paged(wide[:, 2:10], *b.pages()), want)
+    by_head = b.q.transpose(0, 1).contiguous().transpose(0, 1)
+    assert torch.equal(ops.attn_paged(by_head, *b.pages()), want)
+
+
+def test_a_table_far_wider_than_its_sequences():
+    """Capacity in the page table costs no result: a replayed graph's table covers the
+    longest context it may meet."""
+    seqs = [(1, 300), (1, 5), (1, 1000)]
+    a = Batch(seqs, 8, 1, 128, 16, seed=97)
+    w = Batch(seqs, 8, 1, 128, 16, seed=97, extra_width=4000)
+    ref, mag = _attn_ref(a, a.q, 0, None, 128 ** -0.5)
+    for b in (a, w):
+        within(ops.attn_paged(b.q, *b.pages()), ref, _attn_bound(ref, mag, BF16))
+
+
+# -- entries out of range --------------------------------------------------------------
+def _reported():
+    with pytest.raises(_lib.MoeError) as e:
+        ops.check_device_error()
+    assert e.value.code == _lib.MOE_ERR_DEVICE and "page" in str(e.value)
+
+
+@pytest.mark.parametrize("n", [1, 50])
+@pytest.mark.parametrize("page", [-1, 10 ** 6, 2 ** 31 - 1, -2 ** 31])
+def test_pages_out_of_range_are_left_out(page, n):
+    b = Batch([(n, 200), (2, 100)], 8, 1, 64, 16)
+    want = ops.attn_paged(b.q, *b.pages())
+    b.table[0, 3] = page
+    got = ops.attn_paged(b.q, *b.pages())
+    _reported()
+    assert torch.equal(got[n:], want[n:]) and got.isfinite().all()
+    k0, v0 = b.kp.clone(), b.vp.clone()
+    b.table[0, 3] = 0
+    b.table[0, 199 // 16] = page                       # the last new token's page
+    x = randn((b.T, 1, 64), 99)
+    f = torch.zeros(32, dtype=torch.float64, device="cuda")
+    ops.rope_cache(b.q, x, x, *b.pages(), f)
+    _reported()
+    changed = (b.kp != k0).any(-1).any(1)              # [pages, place]
+    live = torch.zeros_like(changed)
+    for s, (m, L) in enumerate(b.seqs):
+        for j in range(L - m, L):
+            if s or j // 16 != 199 // 16:
+                live[b.np_table[s, j // 16], j % 16] = True
+    assert torch.equal(changed, live)
+
+
+@pytest.mark.parametrize("starts,lens", [([0, 60, 52], [200, 100]), ([0, -5, 52], [200, 100]),
+                                         ([7, 50, 2 ** 31 - 1], [200, 100]),
+                                         ([0, 50, 52], [-3, 100]), ([0, 50, 52], [2 ** 31 - 1, 9]),
+                                         ([-2 ** 31, 50, 52], [2 ** 30, -2 ** 31])])
+def test_starts_and_lengths_out_of_range_stay_inside(starts, lens):
+    b = Batch([(50, 200), (2, 100)], 8, 1, 64, 16)
+    b.starts.copy_(torch.tensor(starts))
+    b.lens.copy_(torch.tensor(lens))
+    out = torch.zeros_like(b.q)
+    ops.attn_paged(b.q, *b.pages(), out=out)
+    _reported()
+    assert out.isfinite().all()
+    x = randn((b.T, 1, 64), 99)
+    f = torch.zeros(32, dtype=torch.float64, device="cuda")
+    ops.rope_cache(b.q, x, x, *b.pages(), f, out=out)
+    _reported()
+
+
+# -- streams, graphs ------------------------------------------------------------------
+def _ops_of(b, x, w, w8, ws, freqs):
+    q, s, h = ops.add_rms_norm(x, w, residual=x, fp8=True)
+    y = ops.linear_fp8(q, w8, ws, x_scales=s)
+    y2 = ops.linear_fp8(h, w8, ws)
+    qr = ops.rope_cache(b.q, b.q[:, :2], b.q[:, 2:4], *b.pages(), freqs)
+    return q, s, h, y, y2, qr, ops.attn_paged(qr, *b.pages())
+
+
+def _inputs(seed, seqs):
+    b = Batch(seqs, 8, 2, 64, 16, seed=seed)
+    w8, ws = _weights(300, 512, seed + 5)
+    freqs, _ = ops.rope_freqs(64, 10000.0)
+    return b, randn((37, 512), seed + 7), randn((512,), seed + 8), w8, ws, freqs
+
+
+@pytest.mark.parametrize("seqs", [[(1, 3000), (1, 50)], [(60, 300), (3, 9)]])
+def test_other_streams_and_calls_beside_each_other(seqs):
+    a, c = _inputs(101, seqs), _inputs(201, seqs)
+    want = [_ops_of(*a), _ops_of(*c)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        got = []
+        for s, args in zip(streams, (a, c)):
+            with torch.cuda.stream(s):
+                got.append(_ops_of(*args))
+        torch.cuda.synchronize()
+        for g, w in zip(got, want):
+            for x, y in zip(g, w):
+                assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+    b, x, w, w8, ws, freqs = a
+    s = streams[0]
+    y, h = ops.add_rms_norm(x, w, residual=x, stream=s)
+    z = ops.linear_fp8(h, w8, ws, stream=s)
+    o = ops.attn_paged(want[0][5], *b.pages(), stream=s)
+    torch.cuda.synchronize()
+    assert torch.equal(z, want[0][4]) and torch.equal(o, want[0][6])
+
+
+@pytest.mark.parametrize("seqs", [[(1, 3000), (1, 50)], [(60, 300), (3, 9)]])
+def test_captured_and_replayed(seqs):
+    """Two graphs captured over other inputs, replayed in turn with changed inputs and
+    lengths between, against the same calls made eagerly."""
+    sets = [_inputs(111, seqs), _inputs(121, seqs)]
+    for args in sets:
+        _ops_of(*args)
+    torch.cuda.synchronize()
+    graphs = []
+    for args in sets:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = _ops_of(*args)
+        graphs.append((g, out))
+    for k in range(4):
+        for (g, out), args in zip(graphs, sets):
+            b, x = args[0], args[1]
+            b.q.copy_(randn(b.q.shape, 130 + k))
+            x.copy_(randn(x.shape, 140 + k))
+            if k:
+                b.lens.sub_(1)
+            g.replay()
+        torch.cuda.synchronize()
+        for (g, out), args in zip(graphs, sets):
+            got = [t.clone() for t in out]
+            for x, y in zip(got, _ops_of(*args)):
+                assert torch.equal(x.view(torch.uint8), y.view(torch.uint8)), k
+    ops.check_device_error()
+
+
+# -- a run of them, as a decoder layer uses them -----------------------------------------
+@pytest.mark.parametrize("seqs", [[(1, 90), (1, 33), (1, 1)], [(40, 40), (7, 60)]])
+def test_decoder_layer(seqs):
+    """norm -> query/key/value product -> rotary positions and cache -> attention ->
+    output product -> norm -> router -> experts, every step against the oracle on the
+    step's own inputs."""
+    geom = G.SMALL
+    D, H, HK, DH = geom.d_model, 8, 2, 64
+    b = Batch(seqs, H, HK, DH, 16, seed=151)
+    layer = Layer(geom, 32, 152)
+    x, r = randn((b.T, D), 153), randn((b.T, D), 154)
+    w1, w2, qw, kw = (randn((n,), 155 + i) for i, n in enumerate((D, D, DH, DH)))
+    wqkv, sqkv = _weights((H + 2 * HK) * DH, D, 161)
+    wo, so = _weights(D, H * DH, 163)
+    freqs, m = ops.rope_freqs(DH, 150000.0, 32.0, "yarn")
+    q8, s8, h = ops.add_rms_norm(x, w1, residual=r, fp8=True)
+    qkv = ops.linear_fp8(q8, wqkv, sqkv, x_scales=s8).view(b.T, H + 2 * HK, DH)
+    q = ops.rope_cache(qkv[:, :H], qkv[:, H:H + HK], qkv[:, H + HK:], *b.pages(), freqs,
+                       mscale=m, q_weight=qw, k_weight=kw)
+    o = ops.attn_paged(q, *b.pages())
+    y = ops.linear_fp8(o.view(b.T, H * DH), wo, so)
+    z, h2 = ops.add_rms_norm(y, w2, residual=h)
+    rb = ops.route(z, layer.W, None, geom.routing, geom.norm_topk_prob, geom.top_k,
+                   table=layer.table)
+    e = ops.ffn(layer.pool, rb.slot_refs, rb.scores, z)
+    ops.check_device_error()
+    ref, mag = O.linear(f64(q8), f64(s8), f64(wqkv), f64(sqkv))
+    within(qkv.reshape(b.T, -1), ref, np.abs(ref) * 2.0 ** -8 + mag * (D + 40) * 2.0 ** -23)
+    ref, mag = _attn_ref(b, q, 0, None, DH ** -0.5)
+    # the heads' norms bring |q||k| scale to 2^7
+    within(o, ref, np.abs(ref) * 2.0 ** -8 + (2.0 ** -8 + 2.0 ** -13) * mag)
+    xq, xs = O.quant(f64(o.view(b.T, -1)))
+    ref, mag = O.linear(xq, xs, f64(wo), f64(so))
+    within(y, ref, np.abs(ref) * 2.0 ** -8 + mag * (H * DH + 40) * 2.0 ** -23)
+    assert torch.equal(h2, (y.double() + h.double()).to(BF16))
+    ref = O.rms_norm(f64(h2), f64(w2), 1e-6)
+    within(z, ref, np.abs(ref) * (2.0 ** -8 + 2.0 ** -18))
+    one = ops.ffn_decode(layer.pool, rb.slot_refs[:1], rb.scores[:1], z[:1])
+    assert torch.allclose(e[:1].float(), one.float(), rtol=2e-2, atol=2e-2 * float(one.abs().max()))
