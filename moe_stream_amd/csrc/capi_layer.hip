@@ -25,7 +25,7 @@ int make_kv_args(const moe_kv_view *v, int32_t T, moe::KvArgs *kv) {
   if (v->head_dim <= 0 || v->head_dim % 2 || v->head_dim > moe::kRopeMaxDim)
     return fail(MOE_ERR_INVALID, "head_dim=%d must be even, in [2, %d]", v->head_dim,
                 moe::kRopeMaxDim);
-  if (T < 0 || T > (1 << 24)) return fail(MOE_ERR_INVALID, "T=%d outside [0, 2^24]", T);
+  if (T < 0 || T >= (1 << 24)) return fail(MOE_ERR_INVALID, "T=%d outside [0, 2^24)", T);
   kv->k = static_cast<uint16_t *>(v->k);
   kv->v = static_cast<uint16_t *>(v->v);
   kv->table = v->table;
@@ -50,7 +50,7 @@ int moe_add_rms_norm(const void *x, int64_t x_stride, const void *residual,
                      int32_t width, float eps, void *y, uint8_t *q, float *scales, void *sum,
                      void *stream) {
   if (!is16(dtype)) return fail(MOE_ERR_INVALID, "unknown dtype %d", dtype);
-  if (T < 0) return fail(MOE_ERR_INVALID, "T=%d is negative", T);
+  if (T < 0 || T >= (1 << 24)) return fail(MOE_ERR_INVALID, "T=%d outside [0, 2^24)", T);
   if (width <= 0 || width > moe::kNormMaxWidth)
     return fail(MOE_ERR_INVALID, "width=%d outside [1, %d]", width, moe::kNormMaxWidth);
   if (!(eps >= 0.f)) return fail(MOE_ERR_INVALID, "eps=%g must not be negative", eps);
@@ -90,9 +90,8 @@ static size_t linear_scales_bytes(int32_t T, int32_t K) {
 }
 
 size_t moe_linear_fp8_workspace(int32_t T, int32_t K, int32_t N, int32_t x_dtype) {
-  if (T <= 0 || K <= 0 || N <= 0) return 0;
-  return moe::linear_workspace(T, K, N) +
-         (x_dtype == MOE_DTYPE_E4M3 ? 0 : linear_codes_bytes(T, K) + linear_scales_bytes(T, K));
+  if (T <= 0 || K <= 0 || N <= 0 || x_dtype == MOE_DTYPE_E4M3 || moe::linear_takes_16(T)) return 0;
+  return linear_codes_bytes(T, K) + linear_scales_bytes(T, K);
 }
 
 int moe_linear_fp8(const void *x, int32_t x_dtype, int64_t x_stride, const float *x_scales,
@@ -102,11 +101,13 @@ int moe_linear_fp8(const void *x, int32_t x_dtype, int64_t x_stride, const float
   const bool x8 = x_dtype == MOE_DTYPE_E4M3;
   if (!x8 && !is16(x_dtype)) return fail(MOE_ERR_INVALID, "unknown x dtype %d", x_dtype);
   if (!is16(out_dtype)) return fail(MOE_ERR_INVALID, "unknown output dtype %d", out_dtype);
-  if (T < 0 || T > (1 << 24)) return fail(MOE_ERR_INVALID, "T=%d outside [0, 2^24]", T);
+  if (T < 0 || T >= (1 << 24)) return fail(MOE_ERR_INVALID, "T=%d outside [0, 2^24)", T);
   if (K <= 0 || K % 16 || K > (1 << 20))
     return fail(MOE_ERR_INVALID, "K=%d must be a multiple of 16 in [16, 2^20]", K);
   if (N <= 0 || N > (1 << 22)) return fail(MOE_ERR_INVALID, "N=%d outside [1, 2^22]", N);
   if (T == 0) return MOE_OK;
+  if ((int64_t)T * ((K + moe::kFp8Block - 1) / moe::kFp8Block) >= (1 << 28))
+    return fail(MOE_ERR_INVALID, "T=%d rows of K=%d pass one launch", T, K);
   if (x8 != (x_scales != nullptr))
     return fail(MOE_ERR_INVALID, "x_scales go with an e4m3 x, and only with one");
   if (!x || !w || !w_scales || !y) return fail(MOE_ERR_INVALID, "NULL x/w/w_scales/y");
@@ -125,16 +126,16 @@ int moe_linear_fp8(const void *x, int32_t x_dtype, int64_t x_stride, const float
   a.x_stride = x_stride;
   a.xs = x_scales;
   (void)hipGetLastError();
-  if (!x8) {
+  if (need) {
     uint8_t *codes = reinterpret_cast<uint8_t *>(ws);
     float *scales = reinterpret_cast<float *>(ws + linear_codes_bytes(T, K));
-    ws += linear_codes_bytes(T, K) + linear_scales_bytes(T, K);
     moe::launch_to_fp8(static_cast<const uint16_t *>(x), x_stride, x_dtype, T, K, codes, scales,
                        s);
     MOE_HIP(hipGetLastError());
     a.x = codes;
     a.x_stride = K;
     a.xs = scales;
+    x_dtype = MOE_DTYPE_E4M3;
   }
   a.w = w;
   a.ws = w_scales;
@@ -143,8 +144,7 @@ int moe_linear_fp8(const void *x, int32_t x_dtype, int64_t x_stride, const float
   a.T = T;
   a.K = K;
   a.N = N;
-  a.work = ws;
-  moe::launch_linear(a, out_dtype, s);
+  moe::launch_linear(a, x_dtype, out_dtype, s);
   MOE_HIP(hipGetLastError());
   return MOE_OK;
 }
@@ -209,6 +209,8 @@ int moe_attn_paged(const moe_kv_view *kv, const void *q, int64_t q_token, int64_
                 kv->head_dim, heads / kv->kv_heads);
   if (window < 0) return fail(MOE_ERR_INVALID, "window=%d is negative", window);
   if (T == 0) return MOE_OK;
+  if (!moe::attn_fits(a.kv, heads))
+    return fail(MOE_ERR_UNSUPPORTED, "T=%d rows of %d heads pass one launch", T, heads);
   if (!q || !out) return fail(MOE_ERR_INVALID, "NULL q/out");
   if (!aligned(q, 16) || q_token % 8 || q_head % 8 || !aligned(kv->k, 16) ||
       !aligned(kv->v, 16) || !aligned(out, 16))

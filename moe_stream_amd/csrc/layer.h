@@ -192,20 +192,20 @@ struct AttnArgs {
   float scale;
 };
 bool attn_supported(int dim, int heads, int kv_heads);
+bool attn_fits(const KvArgs &kv, int heads);
 size_t attn_workspace(const KvArgs &kv, int heads);
 void launch_attn(const AttnArgs &a, int dtype, void *ws, hipStream_t s);
 
 // --- 8-bit product (linear_fp8.hip) -----------------------------------------------
 struct LinearArgs {
-  const uint8_t *x, *w;
-  int64_t x_stride;
+  const uint8_t *x, *w;      // (x may hold 16-bit elements, see linear_takes_16)
+  int64_t x_stride;          // elements
   const float *xs, *ws;
   const uint16_t *bias;
   uint16_t *y;
   int32_t T, K, N;
-  void *work;
 };
-size_t linear_workspace(int T, int K, int N);
-void launch_linear(const LinearArgs &a, int out_dtype, hipStream_t s);
+bool linear_takes_16(int T);   // whether x of T rows may come in 16 bits
+void launch_linear(const LinearArgs &a, int x_dtype, int out_dtype, hipStream_t s);
 
 }  // namespace moe
