@@ -410,7 +410,8 @@ int moe_rope_cache(const moe_kv_view *kv, const void *q, int64_t q_token, int64_
  * workspace: at least moe_attn_paged_workspace() bytes, 256-byte aligned; it
  * needs no zeroing.
  */
-size_t moe_attn_paged_workspace(const moe_kv_view *kv, int32_t T, int32_t heads);
+size_t moe_attn_paged_workspace(const moe_kv_view *kv, int32_t T, int32_t heads,
+                                int32_t window);
 int moe_attn_paged(const moe_kv_view *kv, const void *q, int64_t q_token, int64_t q_head,
                    int32_t T, int32_t heads, float scale, int32_t window, const float *sinks,
                    void *out, void *workspace, size_t workspace_bytes, void *stream);

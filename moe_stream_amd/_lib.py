@@ -127,7 +127,7 @@ def _declare(lib):
         "moe_linear_fp8": (C.c_int, [P, I32, I64, P, P, P, P, I32, I32, I32, I32, P, P, SZ, P]),
         "moe_rope_cache": (C.c_int, [C.POINTER(KvView), P, I64, I64, P, I64, I64, P, I64, I64,
                                      I32, I32, P, I32, I32, F, P, P, F, P, P]),
-        "moe_attn_paged_workspace": (SZ, [C.POINTER(KvView), I32, I32]),
+        "moe_attn_paged_workspace": (SZ, [C.POINTER(KvView), I32, I32, I32]),
         "moe_attn_paged": (C.c_int, [C.POINTER(KvView), P, I64, I64, I32, I32, F, I32, P, P, P,
                                      SZ, P]),
         "moe_fill_slots": (C.c_int, [C.POINTER(PoolView), P, I64, I64, P, P, I32, P]),

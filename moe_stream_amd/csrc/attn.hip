@@ -18,18 +18,25 @@
 // sequences are nor how they differ.  A sequence in one part is stored at once;
 // parts of a longer one go to the workspace and a second kernel joins them.
 #include <algorithm>
+#include <type_traits>
 
 #include "layer.h"
 
 namespace moe {
 
+// 16-bit products and conversions.
 template <class T>
-struct Mfma32;
+struct Mat;
 template <>
-struct Mfma32<Bf16> {
-  static constexpr uint32_t kExp = 0x7f80u;   // all ones: not finite
+struct Mat<Bf16> {
+  static constexpr uint32_t kExp = 0x7f807f80u;    // exponents of a pair
+  static constexpr uint32_t kCarry = 0x00800080u;  // carries out of an exponent of ones
   static __device__ __forceinline__ f32x16 mul(u32x4_t a, u32x4_t b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x4 mul(u32x4_t a, u32x4_t b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
                                                    __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
@@ -38,10 +45,15 @@ struct Mfma32<Bf16> {
   }
 };
 template <>
-struct Mfma32<F16> {
-  static constexpr uint32_t kExp = 0x7c00u;
+struct Mat<F16> {
+  static constexpr uint32_t kExp = 0x7c007c00u;
+  static constexpr uint32_t kCarry = 0x04000400u;
   static __device__ __forceinline__ f32x16 mul(u32x4_t a, u32x4_t b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x4 mul(u32x4_t a, u32x4_t b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
                                                   __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
@@ -51,6 +63,20 @@ struct Mfma32<F16> {
   }
 };
 
+// A block of RB x RB results: RB lanes a row, 64 / RB groups of lanes g that hold 4
+// neighbouring keys (or columns of O) in each 4 registers: value e of a lane is at
+//   (4 * 64 / RB) * (e / 4) + 4 g + e % 4.
+template <int RB>
+struct Block;
+template <>
+struct Block<32> {
+  typedef f32x16 acc;
+};
+template <>
+struct Block<16> {
+  typedef f32x4 acc;
+};
+
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kNoMax = -3e38f;   // a row's maximum before its first key: finite, below all scores
 
@@ -58,7 +84,7 @@ struct AttnPlan {
   int tpt;       // tokens a tile
   int hpt;       // heads a token in a tile
   int hchunks;   // tiles that share a key head and its tokens
-  int target;    // items wanted over all key heads; 0: no sequence is cut
+  int target;    // items wanted over all key heads
   int least;     // fewest keys worth a part of their own
   int items;     // items a key head and chunk, at most
   float *po;     // [items][heads' chunks][rows][D] of parts
@@ -68,64 +94,76 @@ struct AttnPlan {
 struct AttnItem {
   int seq, tile, part, parts;
   int first;     // item index of the tile's part 0
+  SeqSpan sp;
   bool live;
 };
 
 // Keys that the tiles of a sequence pass over, at most.
-__device__ __forceinline__ int span_keys(const SeqSpan &sp, int window, int tpt) {
-  return window > 0 ? (int)min((int64_t)sp.len, (int64_t)window + tpt + 63) : sp.len;
+MOE_HD int span_keys(const SeqSpan &sp, int window, int tpt) {
+  return window > 0 ? (int)((int64_t)window + tpt + 63 < sp.len ? (int64_t)window + tpt + 63 : sp.len) : sp.len;
+}
+
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_rows(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+// Sum over this and all lower lanes.
+__device__ __forceinline__ int scan64(int v) {
+  v += dpp_rows<0x111, 0xf>(v);   // row_shr 1, 2, 4, 8
+  v += dpp_rows<0x112, 0xf>(v);
+  v += dpp_rows<0x114, 0xf>(v);
+  v += dpp_rows<0x118, 0xf>(v);
+  v += dpp_rows<0x142, 0xa>(v);   // the row before, then the half before
+  v += dpp_rows<0x143, 0xc>(v);
+  return v;
 }
 
 // The x-th item (by_tile: part 0 of the x-th tile) in order of sequences, tiles and
-// parts; on one wave, 64 sequences a step.  Parts are as long as makes `target` of
-// all of them, so at most target + tiles exist.
+// parts; on one wave, 64 sequences a step.  A part is as long as makes `target` of
+// all of them (in 32 bits, the same in every workgroup), so that at most target / shares
+// + 1 + tiles exist.
 __device__ AttnItem find_item(const KvArgs &kv, const AttnPlan &p, int window, int x,
                               bool by_tile, int lane) {
   const int shares = kv.heads * p.hchunks;
-  int64_t work = 0;
-  if (p.target > 0) {
-    for (int s0 = 0; s0 < kv.n_seqs; s0 += 64) {
-      if (s0 + lane < kv.n_seqs) {
-        const SeqSpan sp = kv_span(kv, s0 + lane);
-        work += (int64_t)((sp.rows + p.tpt - 1) / p.tpt) * span_keys(sp, window, p.tpt);
-      }
-    }
-    for (int m = 1; m < 64; m <<= 1) work += __shfl_xor(work, m);
+  const SeqSpan none = {0, 0, 0, 0, true};
+  SeqSpan sp = none;
+  float work = 0.f;
+  for (int s0 = 0; s0 < kv.n_seqs; s0 += 64) {
+    sp = s0 + lane < kv.n_seqs ? kv_span(kv, s0 + lane) : none;
+    work += (float)((sp.rows + p.tpt - 1) / p.tpt) * (float)span_keys(sp, window, p.tpt);
   }
-  const int64_t span =
-      p.target > 0 ? max((int64_t)p.least, (work * shares + p.target - 1) / p.target) : INT32_MAX;
+  work = group_sum<64>(work) * (float)shares;
+  const int span = max(p.least, (int)fminf(work / (float)p.target, 2e9f) + 1);
   AttnItem it;
   it.live = false;
   int done = 0, done_items = 0;
   for (int s0 = 0; s0 < kv.n_seqs; s0 += 64) {
-    int tiles = 0, parts = 1;
-    if (s0 + lane < kv.n_seqs) {
-      const SeqSpan sp = kv_span(kv, s0 + lane);
-      tiles = (sp.rows + p.tpt - 1) / p.tpt;
-      parts = max(1, (int)((span_keys(sp, window, p.tpt) + span - 1) / span));
-    }
+    if (kv.n_seqs > 64) sp = s0 + lane < kv.n_seqs ? kv_span(kv, s0 + lane) : none;
+    const int tiles = (sp.rows + p.tpt - 1) / p.tpt;
+    const int parts = max(1, (int)(((int64_t)span_keys(sp, window, p.tpt) + span - 1) / span));
     const int n = tiles * parts, c = by_tile ? tiles : n;
-    int inc = c, inc_items = n;
-    for (int m = 1; m < 64; m <<= 1) {
-      const int u = __shfl_up(inc, m), v = __shfl_up(inc_items, m);
-      if (lane >= m) inc += u, inc_items += v;
-    }
+    const int inc_items = scan64(n), inc = by_tile ? scan64(c) : inc_items;
     const uint64_t past = __ballot(x < done + inc);
     if (past) {
       const int l = __ffsll((unsigned long long)past) - 1;
-      const int i = x - done - __shfl(inc - c, l);
+      auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+      const int i = x - done - of(inc - c);
       it.seq = s0 + l;
-      it.parts = __shfl(parts, l);
+      it.parts = of(parts);
       it.tile = by_tile ? i : i / it.parts;
       it.part = by_tile ? 0 : i % it.parts;
-      it.first = done_items + __shfl(inc_items - n, l) + it.tile * it.parts;
+      it.first = done_items + of(inc_items - n) + it.tile * it.parts;
+      it.sp.first = of(sp.first);
+      it.sp.rows = of(sp.rows);
+      it.sp.len = of(sp.len);
+      it.sp.base = of(sp.base);
+      it.sp.ok = of(sp.ok);
       // (sums that wrapped, of starts that make no sense, end here)
-      it.live = i >= 0 && it.tile < __shfl(tiles, l) && it.first >= 0 &&
-                it.first <= p.items - it.parts;
+      it.live = i >= 0 && it.tile < of(tiles) && it.first >= 0 && it.first <= p.items - it.parts;
       break;
     }
-    done += __shfl(inc, 63);
-    done_items += __shfl(inc_items, 63);
+    done += __builtin_amdgcn_readlane(inc, 63);
+    done_items += __builtin_amdgcn_readlane(inc_items, 63);
   }
   return it;
 }
@@ -153,21 +191,31 @@ __device__ __forceinline__ AttnTile attn_tile(const SeqSpan &sp, int tile, int t
   return t;
 }
 
-__device__ __forceinline__ float other_half(float v) {   // the value of lane ^ 32
-  const uint32_t b = __float_as_uint(v);
-  const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
-  return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+// Over the groups of lanes that hold one row.
+template <int RB, class F>
+__device__ __forceinline__ float over_groups(float v, F f) {
+  uint32_t b = __float_as_uint(v);
+  auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+  v = f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  if (RB == 16) {
+    b = __float_as_uint(v);
+    r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+    v = f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  }
+  return v;
 }
 
 // 16-byte piece c of row `row` stands at piece c ^ swz of that row.  K is read 16
-// rows a phase at one piece, V 4 rows at four neighbouring ones.
+// rows a phase at one piece; V 4 rows a phase at four neighbouring pieces (RB 32) or
+// 8 rows at two.
 template <int D>
 __device__ __forceinline__ int swz_k(int row) {
   return D == 128 ? (row & 15) : ((row >> 1) & 7);
 }
-template <int D>
+template <int D, int RB>
 __device__ __forceinline__ int swz_v(int row) {
-  return D == 128 ? (row & 3) << 2 : ((row >> 1) & 1) << 2;
+  if (RB == 32) return D == 128 ? (row & 3) << 2 : ((row >> 1) & 1) << 2;
+  return D == 128 ? (row & 7) << 1 : ((row >> 1) & 3) << 1;
 }
 
 typedef __attribute__((address_space(3))) void lds_void;
@@ -182,18 +230,37 @@ __device__ __forceinline__ uint64_t bit_range(int a, int b) {
   return (~0ull >> (64 - (b - a))) << a;
 }
 
-// QW waves side by side on 32 rows each share the tiles of keys; or KW waves take
-// every KW-th tile for the same 32 rows and are joined at the end.
-template <class T, int D, int QW, int KW, int BK>
-__global__ __launch_bounds__(64 * QW * KW, QW > 1 ? 2 : 1) void attn_kernel(AttnArgs a, AttnPlan p) {
+// What rows without a page read instead, a load's worth.
+__device__ const uint4 g_no_page[64] = {};
+
+// QW waves side by side on RB rows each share the tiles of keys; or KW waves take
+// every KW-th tile for the same RB rows and are joined at the end.
+//
+// A step of the loop interleaves, instruction by instruction, the scores of tile i + 1
+// with the exponentials of tile i, and the output of tile i with the maxima of tile
+// i + 1: a wave's vector instructions run beside its own matrix instruction, but those of
+// two waves of a SIMD do not (measured: a wave of products alone beside a wave of
+// multiply-adds alone takes longer than one after the other), so the pairs are made here.
+template <class T, int D, int RB, int QW, int KW, int BK>
+__global__ __launch_bounds__(64 * QW * KW, QW > 1 ? 2 : 1) void attn_kernel(AttnArgs a,
+                                                                          AttnPlan p) {
   static_assert(QW == 1 || KW == 1, "one of the two");
-  using M = Mfma32<T>;
-  constexpr int kRows = 32 * QW;
+  using M = Mat<T>;
+  using Acc = typename Block<RB>::acc;
+  using Yes = std::true_type;
+  using No = std::false_type;
+  constexpr int NG = 64 / RB;                    // groups of lanes
+  constexpr int AE = RB / NG;                    // values of a block a lane
+  constexpr int kRows = RB * QW;
   constexpr int kTileBytes = BK * D * 2;         // of K, and of V
   constexpr int kRowsPerLoad = 1024 / (2 * D);   // rows that one wave load brings
   constexpr int kLoads = kTileBytes / 1024 / QW; // a wave's loads of K, and of V
   constexpr int kPieces = D / 8;                 // 16-byte pieces a row
-  __shared__ __align__(1024) char lds[KW * 4 * kTileBytes];   // [KW][2][K tile, V tile]
+  constexpr int kSteps = BK / (8 * NG);          // steps of 8 NG keys of the second product
+  // Two tiles of K and of V a key wave, each an array of its own: loads to one are under
+  // way while another is read, which the compiler waits for unless it tells them apart.
+  __shared__ __align__(1024) char lds_k0[KW * kTileBytes], lds_k1[KW * kTileBytes];
+  __shared__ __align__(1024) char lds_v0[KW * kTileBytes], lds_v1[KW * kTileBytes];
   __shared__ unsigned long long all_bad;
   const KvArgs &kv = a.kv;
   const int lane = threadIdx.x & 63;
@@ -201,31 +268,14 @@ __global__ __launch_bounds__(64 * QW * KW, QW > 1 ? 2 : 1) void attn_kernel(Attn
   const int wq = QW > 1 ? wave : 0, wk = KW > 1 ? wave : 0;
   const int shares = kv.heads * p.hchunks;
   const int share = blockIdx.x % shares;
-  // the last items first: a sequence's later rows see the most keys
-  const int x = gridDim.x / shares - 1 - blockIdx.x / shares;
+  // many rows: the last items first, since a sequence's later rows see the most keys
+  const int x = QW > 1 ? gridDim.x / shares - 1 - blockIdx.x / shares : blockIdx.x / shares;
   const AttnItem it = find_item(kv, p, a.window, x, false, lane);
   if (!it.live) return;
-  const SeqSpan sp = kv_span(kv, it.seq);
+  const SeqSpan sp = it.sp;
   if (!sp.ok && threadIdx.x == 0) flag_error_bits(kErrBadBatch);
   const AttnTile tl = attn_tile(sp, it.tile, p.tpt, a.window);
   const int hk = share / p.hchunks;
-  const int group = a.heads / kv.heads;
-  const int h0 = (share % p.hchunks) * p.hpt;
-
-  // this lane's row
-  const int r = wq * 32 + (lane & 31), hi = lane >> 5;
-  const int tok = r / p.hpt, hh = h0 + r % p.hpt;
-  const bool row_live = tok < tl.tokens && hh < group;
-  const int t = tl.row0 + tok, h = hk * group + hh;
-  int lo_key = 0, hi_key = 0;
-  if (row_live) seen_keys(tl.pos0 + tok, sp.len, a.window, &lo_key, &hi_key);
-  u32x4_t q[D / 16];
-#pragma unroll
-  for (int st = 0; st < D / 16; ++st) {
-    q[st] = (u32x4_t){0, 0, 0, 0};
-    if (row_live)
-      q[st] = *reinterpret_cast<const u32x4_t *>(a.q + t * a.q_st + h * a.q_sh + 16 * st + 8 * hi);
-  }
 
   // this part's keys
   const int n_keys = max(0, tl.end - tl.start);
@@ -238,131 +288,216 @@ __global__ __launch_bounds__(64 * QW * KW, QW > 1 ? 2 : 1) void attn_kernel(Attn
     const int j = j0 + lane;
     return lane < BK && j < k1 ? table[j >> kv.page_shift] : -1;
   };
-  auto valid_of = [&](int entry) { return __ballot(entry >= 0 && entry < kv.n_pages); };
-  char *const mine = lds + wk * 4 * kTileBytes;
-  // Rows of one load lie in one page (pages hold 16 rows or more, and tiles start at
-  // a multiple of 32); a row with no page is read from page 0 and not used.
-  auto fetch = [&](int j0, int entry, int buf) {
-    char *const kb = mine + buf * 2 * kTileBytes, *const vb = kb + kTileBytes;
-    const int sub = lane / kPieces, piece = lane % kPieces;
+  auto k_tile = [&](auto odd) { return (decltype(odd)::value ? lds_k1 : lds_k0) + wk * kTileBytes; };
+  auto v_tile = [&](auto odd) { return (decltype(odd)::value ? lds_v1 : lds_v0) + wk * kTileBytes; };
+  // Lane j: where key j0 + j's row of K starts, or that of V.  Rows of one load lie in
+  // one page (pages hold 16 rows or more, and tiles start at a multiple of 32), so a load
+  // goes from its first row's address, and the lanes' places in it are the wave's own.
+  auto rows_of = [&](int j0, int entry) {
+    return page_row(entry, kv.n_pages, kv.heads, hk, kv.page_shift, j0 + lane, D);
+  };
+  auto start_of = [&](const uint16_t *pages, int64_t row) {
+    return reinterpret_cast<uint64_t>(row >= 0 ? pages + row
+                                               : reinterpret_cast<const uint16_t *>(g_no_page));
+  };
+  const int sub = lane / kPieces, piece = lane % kPieces;
+  auto fetch = [&](bool is_v, uint64_t start, int i, char *to) __attribute__((always_inline)) {
+    const int n = i * QW + wq, row = n * kRowsPerLoad;
+    const int swz = is_v ? swz_v<D, RB>(row + sub) : swz_k<D>(row + sub);
+    const uint32_t at = sub * (2 * D) + (piece ^ swz) * 16;
+    const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)start, row);
+    const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(start >> 32), row);
+    const char *src = reinterpret_cast<const char *>(((uint64_t)hi << 32) | lo) + at;
+    __builtin_amdgcn_global_load_lds((global_void *)src, (lds_void *)(to + n * 1024), 16, 0, 0);
+  };
+
+  // this lane's row
+  const int group = a.heads / kv.heads;
+  const int h0 = (share % p.hchunks) * p.hpt;
+  const int r = wq * RB + lane % RB, g = lane / RB;
+  const int tok = r / p.hpt, hh = h0 + r % p.hpt;
+  const bool row_live = tok < tl.tokens && hh < group;
+  const int t = tl.row0 + tok, h = hk * group + hh;
+  u32x4_t q[D / (8 * NG)];
+  auto load_q = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int n = i * QW + wq, row = n * kRowsPerLoad;
-      int e = __builtin_amdgcn_readlane(entry, row);
-      e = e >= 0 && e < kv.n_pages ? e : 0;
-      const int64_t base =
-          page_row(e, kv.n_pages, kv.heads, hk, kv.page_shift, j0 + row, D) + sub * D;
-      const uint16_t *gk = kv.k + base + (piece ^ swz_k<D>(row + sub)) * 8;
-      const uint16_t *gv = kv.v + base + (piece ^ swz_v<D>(row + sub)) * 8;
-      __builtin_amdgcn_global_load_lds((global_void *)gk, (lds_void *)(kb + n * 1024), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((global_void *)gv, (lds_void *)(vb + n * 1024), 16, 0, 0);
+    for (int st = 0; st < D / (8 * NG); ++st) {
+      q[st] = (u32x4_t){0, 0, 0, 0};
+      if (row_live)
+        q[st] = *reinterpret_cast<const u32x4_t *>(a.q + t * a.q_st + h * a.q_sh + 8 * NG * st +
+                                                   8 * g);
     }
   };
-  auto landed = [&] {   // this tile's bytes are in LDS, the other buffer is free
-    if (QW > 1) {
-      __syncthreads();
-    } else {
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-      __builtin_amdgcn_sched_barrier(0);
-    }
+  int lo_key = 0, hi_key = 0;
+  if (row_live) seen_keys(tl.pos0 + tok, sp.len, a.window, &lo_key, &hi_key);
+
+  // Keys of a tile that have a page; whether every row sees all of it; the keys that
+  // this lane's row sees.
+  auto valid_of = [&](int entry) { return __ballot(entry >= 0 && entry < kv.n_pages); };
+  auto is_full = [&](int j0, uint64_t valid) {
+    return j0 >= tl.full0 && j0 + BK <= tl.full1 &&
+           (uint64_t)(valid << (64 - BK)) >> (64 - BK) == ~0ull >> (64 - BK);
+  };
+  auto seen_of = [&](int j0, uint64_t valid) __attribute__((always_inline)) {
+    if ((valid | ~bit_range(0, min(BK, k1 - j0))) != ~0ull && lane == 0)
+      flag_error_bits(kErrBadBatch);
+    return bit_range(lo_key - j0, hi_key - j0) & valid;
   };
 
   const float c = fmaxf(a.scale * kLog2e, 1e-37f);
   float m = kNoMax, l = 0.f;
-  f32x16 o[D / 32];
+  Acc o[D / RB];
+  u32x4_t pf[kSteps];
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i)
+  for (int i = 0; i < D / RB; ++i)
 #pragma unroll
-    for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
+    for (int e = 0; e < AE; ++e) o[i][e] = 0.f;
 
-  int j0 = k0 + wk * BK;
-  int entry = j0 < k1 ? entry_of(j0) : -1, buf = 0;
-  if (j0 < k1) fetch(j0, entry, 0);
-  int entry_next = j0 + BK * KW < k1 ? entry_of(j0 + BK * KW) : -1;
-  for (; j0 < k1; j0 += BK * KW, buf ^= 1) {
-    landed();
-    const uint64_t valid = valid_of(entry);
-    const bool in_full = j0 >= tl.full0 && j0 + BK <= tl.full1;
-    const bool full = in_full && (uint64_t)(valid << (64 - BK)) >> (64 - BK) == ~0ull >> (64 - BK);
-    entry = entry_next;
-    if (j0 + BK * KW < k1) {
-      fetch(j0 + BK * KW, entry, buf ^ 1);
-      entry_next = j0 + 2 * BK * KW < k1 ? entry_of(j0 + 2 * BK * KW) : -1;
+  constexpr int kVals = BK / NG;                           // scores of a tile a lane
+  constexpr int kMulS = BK / RB * (D / (8 * NG));          // products of the scores
+  constexpr int kMulO = kSteps * (D / RB);                 // and of the output
+  constexpr int kAheadK = 4, kAheadV = 3;                  // operands read ahead
+  typedef Acc Scores[BK / RB];
+
+  // Where a lane reads in a tile, but for the operand's number: the pieces' permutation is
+  // the same in every block of rows, so the number only flips bits of it.  (Held as one
+  // value each: through long sums the compiler loses sight of which array is read.)
+  const int i16 = lane & 15;
+  int k_at = lane % RB * (2 * D) + (g ^ swz_k<D>(lane % RB)) * 16;
+  int v_at = (4 * g + i16 / 4) * (2 * D) + (i16 & 1) * 8 +
+             (((RB == 32 ? 2 * ((lane >> 4) & 1) : 0) + (i16 & 3) / 2) ^
+              swz_v<D, RB>(4 * g + i16 / 4)) * 16;
+  asm("" : "+v"(k_at), "+v"(v_at));
+  auto k_operand = [&](const char *kb, int u) __attribute__((always_inline)) {
+    const int b = u / (D / (8 * NG)), st = u % (D / (8 * NG));
+    return *reinterpret_cast<const u32x4_t *>(kb + (k_at ^ (NG * st * 16)) + RB * b * (2 * D));
+  };
+  // 16 lanes read 4 keys of 16 columns, and lane i gets column i of them.
+  auto v_operand = [&](const char *vb, int u) __attribute__((always_inline)) {
+    const int st = u / (D / RB), d = u % (D / RB);
+    u32x4_t vf;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const s16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) s16x4 *)(vb + (v_at ^ (d * RB * 2)) +
+                                                      (2 * st + k) * 4 * NG * (2 * D)));
+      const uint2 x2 = __builtin_bit_cast(uint2, w);
+      vf[2 * k] = x2.x;
+      vf[2 * k + 1] = x2.y;
     }
-    const char *const kb = mine + buf * 2 * kTileBytes;
-    char *const vb = mine + buf * 2 * kTileBytes + kTileBytes;
-
-    uint64_t vis = 0;   // keys that this lane's row sees, where the tile is not full
-    if (!full) {
-      if ((valid | ~bit_range(0, k1 - j0)) != ~0ull && lane == 0) flag_error_bits(kErrBadBatch);
-      vis = bit_range(lo_key - j0, min(hi_key, k1) - j0) & valid;
-      // 0 * v is not 0 where v is not finite: such values, and what pages hold past the
-      // sequence, become zero, and rows that do see one become NaN.
-      uint64_t bad = 0;
-      constexpr int kIters = BK * kPieces / (64 * QW);
+    return vf;
+  };
+  // Tile i's weights from its scores sc, beside tile i + 1's scores into sn (next).
+  // A lane's row stands against keys 4 NG (e / 4) + 4 g + e % 4 of the tile.
+  // The loads of what comes next, one after the other, go between the first products.
+  auto weigh = [&](Scores &sc, Scores &sn, const char *kb, auto now, auto next, auto load)
+      __attribute__((always_inline)) {
+    constexpr bool kNow = decltype(now)::value, kNext = decltype(next)::value;
+    constexpr int kEach = (2 * kLoads + kMulS - 1) / kMulS;   // loads a product
+    u32x4_t kf[kAheadK];
+    if constexpr (kNext) {
 #pragma unroll
-      for (int i = 0; i < kIters; ++i) {
-        const int at = (i * QW + wq) * 64 + lane, row = at / kPieces;
-        u32x4_t w = *reinterpret_cast<u32x4_t *>(vb + at * 16);
-        const bool use = (valid >> row) & 1;
-        bool b = false;
+      for (int u = 0; u < kAheadK && u < kMulS; ++u) kf[u] = k_operand(kb, u);
+    }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t x0 = M::kExp, x1 = M::kExp << 16;
-          uint32_t keep = ~0u;
-          if ((w[e] & x0) == x0) keep &= 0xffff0000u;
-          if ((w[e] & x1) == x1) keep &= 0x0000ffffu;
-          b |= keep != ~0u;
-          w[e] &= use ? keep : 0u;
+    for (int u = 0; u < kMulS; ++u) {
+      if constexpr (kNow) {
+#pragma unroll
+        for (int k = 2 * (u * (kVals / 2) / kMulS); k < 2 * ((u + 1) * (kVals / 2) / kMulS);
+             k += 2) {
+          // rounded to the values' type for the matrix unit: half a step of a weight
+          const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[k / AE][k % AE], c, -m));
+          const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[k / AE][k % AE + 1], c, -m));
+          uint32_t w = M::pack(p0, p1);
+          l += p0 + p1;
+          asm volatile("" : "+v"(w), "+v"(l));   // (taken here, not where they are used)
+          pf[k / 8][(k % 8) / 2] = w;
         }
-        b &= use;
-        if (b || !use) *reinterpret_cast<u32x4_t *>(vb + at * 16) = w;
-        const uint64_t lanes = __ballot(b);
-#pragma unroll
-        for (int k = 0; k < 64 / kPieces; ++k)
-          if ((lanes >> (k * kPieces)) & ((1u << kPieces) - 1))
-            bad |= 1ull << ((i * QW + wq) * (64 / kPieces) + k);
       }
-      if (QW > 1) {   // each wave looked at a share of the rows
-        if (threadIdx.x == 0) all_bad = 0;
-        __syncthreads();
-        if (lane == 0 && bad) atomicOr(&all_bad, (unsigned long long)bad);
-        __syncthreads();
-        bad = all_bad;
-      }
-      if (bad & vis) l = __builtin_nanf("");
-    }
-
-    // S^T: this lane's row against keys 32 kb + 8 (r / 4) + 4 hi + r % 4
-    f32x16 s[BK / 32];
+      if constexpr (kNext) {
+        const int b = u / (D / (8 * NG)), st = u % (D / (8 * NG));
+        sn[b] = M::mul(kf[u % kAheadK], q[st], st == 0 ? Acc{} : sn[b]);
+        if (u + kAheadK < kMulS) kf[u % kAheadK] = k_operand(kb, u + kAheadK);
 #pragma unroll
-    for (int b = 0; b < BK / 32; ++b) {
-      const int row = 32 * b + (lane & 31);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) s[b][e] = 0.f;
-#pragma unroll
-      for (int st = 0; st < D / 16; ++st) {
-        const u32x4_t kf = *reinterpret_cast<const u32x4_t *>(
-            kb + row * (2 * D) + ((2 * st + hi) ^ swz_k<D>(row)) * 16);
-        s[b] = M::mul(kf, q[st], s[b]);
+        for (int k = u * kEach; k < (u + 1) * kEach && k < 2 * kLoads; ++k) load(k);
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
-    if (!full) {
-      const uint64_t v = vis >> (4 * hi);
+  };
+  auto hide = [&](Scores &sn, uint64_t vis) __attribute__((always_inline)) {
+    const uint64_t v = vis >> (4 * g);
 #pragma unroll
-      for (int b = 0; b < BK / 32; ++b)
+    for (int b = 0; b < BK / RB; ++b)
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (!((v >> (32 * b + 8 * (e / 4) + e % 4)) & 1)) s[b][e] = -INFINITY;
+      for (int e = 0; e < AE; ++e)
+        if (!((v >> (RB * b + 4 * NG * (e / 4) + e % 4)) & 1)) sn[b][e] = -INFINITY;
+  };
+  // The output of tile i, keys in the order in which the scores left them (a step takes
+  // two runs of 4 keys a group), beside the largest next score.
+  auto output = [&](const char *vb, Scores &sn, auto next) __attribute__((always_inline)) {
+    constexpr bool kNext = decltype(next)::value;
+    u32x4_t vf[kAheadV];
+    float mx = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < kAheadV && u < kMulO; ++u) vf[u] = v_operand(vb, u);
+#pragma unroll
+    for (int u = 0; u < kMulO; ++u) {
+      const int st = u / (D / RB), d = u % (D / RB);
+      o[d] = M::mul(vf[u % kAheadV], pf[st], o[d]);
+      if (u + kAheadV < kMulO) vf[u % kAheadV] = v_operand(vb, u + kAheadV);
+      if constexpr (kNext) {
+#pragma unroll
+        for (int k = u * kVals / kMulO; k < (u + 1) * kVals / kMulO; ++k)
+          mx = fmaxf(mx, sn[k / AE][k % AE]);
+      }
+      asm volatile("" : "+v"(mx));   // (here, between the products)
+      __builtin_amdgcn_sched_barrier(0);
     }
-    float mx = s[0][0];
+    return mx;
+  };
+  // Where a row does not see the whole tile, 0 * v has to be 0 whatever v is: values that
+  // are not finite become zero in LDS first, and rows that do see one become NaN.
+  auto scrub = [&](char *vb, uint64_t vis) __attribute__((always_inline)) {
+    constexpr int kIters = BK * kPieces / (64 * QW);
+    uint64_t bad = 0;   // keys with such a value
+    if (QW > 1 && threadIdx.x == 0) all_bad = 0;
+    if (QW > 1) __syncthreads();
+#pragma unroll 1
+    for (int i = 0; i < kIters; ++i) {
+      const int at = (i * QW + wq) * 64 + lane;
+      u32x4_t w = *reinterpret_cast<u32x4_t *>(vb + at * 16);
+      uint32_t any = 0;
 #pragma unroll
-    for (int b = 0; b < BK / 32; ++b)
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t odd = ((w[e] & M::kExp) + M::kCarry) & 0x80008000u;   // sign bits
+        any |= odd;
+        w[e] &= ~((odd >> 15) * 0xffffu);
+      }
+      const uint64_t lanes = __ballot(any != 0);
+      if (lanes == 0) continue;
+      *reinterpret_cast<u32x4_t *>(vb + at * 16) = w;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[b][e]);
-    mx = fmaxf(mx, other_half(mx)) * c;
-    // The maximum moves only when a score passes it by 2^8: exponentials up to that
-    // are as exact, and most tiles rescale nothing.  A row's own scores decide.
+      for (int k = 0; k < 64 / kPieces; ++k)
+        if ((lanes >> (k * kPieces)) & ((1u << kPieces) - 1))
+          bad |= 1ull << ((i * QW + wq) * (64 / kPieces) + k);
+    }
+    if (QW > 1) {   // each wave looked at a share of the rows
+      if (lane == 0 && bad) atomicOr(&all_bad, (unsigned long long)bad);
+      __syncthreads();
+      bad = all_bad;
+    }
+    if (bad & vis) l = __builtin_nanf("");
+  };
+  auto largest = [&](Scores &sn) __attribute__((always_inline)) {
+    float mx = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kVals; ++k) mx = fmaxf(mx, sn[k / AE][k % AE]);
+    return mx;
+  };
+  // The maximum moves only when a score passes it by 2^8: exponentials up to that are
+  // as exact, and most tiles rescale nothing.  A row's own scores decide.
+  auto rescale = [&](float mx) __attribute__((always_inline)) {
+    mx = over_groups<RB>(mx, [](float u, float v) { return fmaxf(u, v); }) * c;
     const bool moves = mx > m + 8.f;
     if (__any(moves)) {
       const float m1 = moves ? mx : m;
@@ -370,86 +505,128 @@ __global__ __launch_bounds__(64 * QW * KW, QW > 1 ? 2 : 1) void attn_kernel(Attn
       m = m1;
       l *= f;
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i)
+      for (int i = 0; i < D / RB; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) o[i][e] *= f;
+        for (int e = 0; e < AE; ++e) o[i][e] *= f;
     }
-    u32x4_t pf[BK / 16];
-    float sum = 0.f;
-#pragma unroll
-    for (int b = 0; b < BK / 32; ++b)
-#pragma unroll
-      for (int e = 0; e < 16; e += 2) {
-        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[b][e], c, -m));
-        const float p1 = __builtin_amdgcn_exp2f(fmaf(s[b][e + 1], c, -m));
-        sum += p0 + p1;
-        // rounded to the values' type for the matrix unit: half a step of a weight
-        pf[2 * b + e / 8][(e % 8) / 2] = M::pack(p0, p1);
-      }
-    l += sum;
-    // O^T: a step of 16 keys, in the order in which S^T left them
-#pragma unroll
-    for (int st = 0; st < BK / 16; ++st) {
-#pragma unroll
-      for (int d = 0; d < D / 32; ++d) {
-        // lanes 16 g + i of a half read 4 keys of 16 columns, lane i column i of them
-        const int i = lane & 15;
-        const int piece = 4 * d + 2 * ((lane >> 4) & 1) + (i & 3) / 2;
-        u32x4_t vf;
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int row = 16 * st + 8 * k + 4 * hi + i / 4;
-          const char *at = vb + row * (2 * D) + (piece ^ swz_v<D>(row)) * 16 + (i & 1) * 8;
-          const s16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (__attribute__((address_space(3))) s16x4 *)(at));
-          const uint2 u = __builtin_bit_cast(uint2, w);
-          vf[2 * k] = u.x;
-          vf[2 * k + 1] = u.y;
-        }
-        o[d] = M::mul(vf, pf[st], o[d]);
-      }
-    }
-  }
-  l += other_half(l);
+  };
 
-  if (KW > 1) {   // the waves' keys joined on wave 0, one after the other
-    for (int w = 1; w < KW; ++w) {
-      __syncthreads();
-      float *const box = reinterpret_cast<float *>(lds);
-      if (wk == w) {
+  // This wave's tiles: n of them, tile i at key_of(i).  Before step i, the keys of tile
+  // i + 1 and the values of tile i land; what step i - 1 read is free for the next.
+  auto key_of = [&](int i) { return k0 + (wk + i * KW) * BK; };
+  const int n = (max(0, k1 - k0 - wk * BK) + BK * KW - 1) / (BK * KW);
+  int e0 = n > 0 ? entry_of(key_of(0)) : -1;
+  const int e1 = n > 1 ? entry_of(key_of(1)) : -1;
+  load_q();
+  // A workgroup barrier alone does not wait for loads that go to LDS.  (As a builtin, so
+  // that the compiler knows of the wait and adds none of its own before the reads.)
+  auto landed = [&]() __attribute__((always_inline)) {
+    issue_order_fence();
+    __builtin_amdgcn_s_waitcnt(loads_left(0));
+    if (QW > 1) __syncthreads();
+    issue_order_fence();
+  };
+  Scores s0, s1;
+  bool full = true;
+  uint64_t vis = 0, valid_next = 0;
+  int64_t rows = 0;   // lane j: row j of tile i + 1
+  if (n > 0) {
+    rows = rows_of(key_of(0), e0);
+    const uint64_t kp = start_of(kv.k, rows), vp = start_of(kv.v, rows);
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) box[(i * 16 + e) * 64 + lane] = o[i][e];
-        box[D / 2 * 64 + lane] = m;
-        box[D / 2 * 64 + 64 + lane] = l;
-      }
-      __syncthreads();
-      if (wk == 0) {
-        const float m2 = box[D / 2 * 64 + lane], l2 = box[D / 2 * 64 + 64 + lane];
-        const float mm = fmaxf(m, m2);
-        const float f = __builtin_amdgcn_exp2f(m - mm), g = __builtin_amdgcn_exp2f(m2 - mm);
-        m = mm;
-        l = l * f + l2 * g;
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            o[i][e] = o[i][e] * f + box[(i * 16 + e) * 64 + lane] * g;
-      }
+    for (int k = 0; k < kLoads; ++k) fetch(false, kp, k, k_tile(No()));
+    landed();
+    const uint64_t valid = valid_of(e0);
+    rows = rows_of(key_of(1), e1);
+    const uint64_t kp1 = start_of(kv.k, rows);
+    valid_next = valid_of(e1);
+    e0 = n > 2 ? entry_of(key_of(2)) : -1;
+    weigh(s0, s0, k_tile(No()), No(), Yes(), [&](int k) __attribute__((always_inline)) {
+      if (k < kLoads) fetch(true, vp, k, v_tile(No()));
+      else if (n > 1) fetch(false, kp1, k - kLoads, k_tile(Yes()));
+    });
+    full = is_full(key_of(0), valid);
+    if (!full) hide(s0, vis = seen_of(key_of(0), valid));
+    rescale(largest(s0));
+  }
+  auto step = [&](int i, Scores &sc, Scores &sn, auto odd, auto next)
+      __attribute__((always_inline)) {
+    constexpr bool kNext = decltype(next)::value;
+    using Other = std::bool_constant<!decltype(odd)::value>;   // tile i + 1's buffers
+    landed();
+    const uint64_t valid = valid_next;
+    uint64_t vp = 0, kp = 0;
+    const bool more = i + 2 < n;
+    if constexpr (kNext) {
+      vp = start_of(kv.v, rows);
+      rows = rows_of(key_of(i + 2), e0);
+      kp = start_of(kv.k, rows);
+      valid_next = valid_of(e0);
+      e0 = i + 3 < n ? entry_of(key_of(i + 3)) : -1;
     }
+    if (!full) scrub(v_tile(odd), vis);
+    weigh(sc, sn, k_tile(Other()), Yes(), next, [&](int k) __attribute__((always_inline)) {
+      if (k < kLoads) fetch(true, vp, k, v_tile(Other()));
+      else if (more) fetch(false, kp, k - kLoads, k_tile(odd));
+    });
+    bool full_next = true;
+    uint64_t vis_next = 0;
+    if constexpr (kNext) {
+      full_next = is_full(key_of(i + 1), valid);
+      if (!full_next) hide(sn, vis_next = seen_of(key_of(i + 1), valid));
+    }
+    const float mx = output(v_tile(odd), sn, next);
+    if constexpr (kNext) rescale(mx);
+    full = full_next;
+    vis = vis_next;
+  };
+  int i = 0;
+  for (; i + 2 < n; i += 2) {
+    step(i, s0, s1, No(), Yes());
+    step(i + 1, s1, s0, Yes(), Yes());
+  }
+  if (i + 1 < n) {
+    step(i, s0, s1, No(), Yes());
+    step(i + 1, s1, s0, Yes(), No());
+  } else if (i < n) {
+    step(i, s0, s1, No(), No());
+  }
+  l = over_groups<RB>(l, [](float u, float v) { return u + v; });
+
+  if (KW > 1) {   // the waves' keys joined on wave 0, in order
+    constexpr int kBox = D / NG * 64;
+    float *const box = reinterpret_cast<float *>(lds_k0) + lane;
+    float2 *const stat = reinterpret_cast<float2 *>(lds_v0) + lane;
+    static_assert((KW - 1) * kBox * 4 <= KW * kTileBytes, "the boxes fit the tiles");
+    __syncthreads();
+    if (wk > 0) {
+#pragma unroll
+      for (int i = 0; i < D / NG; ++i) box[(wk - 1) * kBox + i * 64] = o[i / AE][i % AE];
+      stat[(wk - 1) * 64] = make_float2(m, l);
+    }
+    __syncthreads();
     if (wk != 0) return;
+    for (int w = 0; w < KW - 1; ++w) {
+      const float2 s2 = stat[w * 64];
+      const float mm = fmaxf(m, s2.x);
+      const float f = __builtin_amdgcn_exp2f(m - mm), f2 = __builtin_amdgcn_exp2f(s2.x - mm);
+      m = mm;
+      l = l * f + s2.y * f2;
+#pragma unroll
+      for (int i = 0; i < D / NG; ++i)
+        o[i / AE][i % AE] = o[i / AE][i % AE] * f + box[w * kBox + i * 64] * f2;
+    }
   }
   if (!row_live) return;
   if (it.parts > 1) {
     const int64_t at = ((int64_t)x * shares + share) * kRows + r;
-    if (hi == 0) p.pml[at] = make_float2(m, l);
+    if (g == 0) p.pml[at] = make_float2(m, l);
     if (l == 0.f) return;   // no key of this part is seen
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i)
+    for (int i = 0; i < D / RB; ++i)
 #pragma unroll
-      for (int e = 0; e < 16; e += 4)
-        *reinterpret_cast<f32x4 *>(p.po + at * D + 32 * i + 2 * e + 4 * hi) =
+      for (int e = 0; e < AE; e += 4)
+        *reinterpret_cast<f32x4 *>(p.po + at * D + RB * i + NG * e + 4 * g) =
             (f32x4){o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]};
     return;
   }
@@ -462,92 +639,98 @@ __global__ __launch_bounds__(64 * QW * KW, QW > 1 ? 2 : 1) void attn_kernel(Attn
   f = l == 0.f ? 0.f : f / l;
   uint16_t *const out = a.out + ((int64_t)t * a.heads + h) * D;
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i)
+  for (int i = 0; i < D / RB; ++i)
 #pragma unroll
-    for (int e = 0; e < 16; e += 4)
-      *reinterpret_cast<uint2 *>(out + 32 * i + 2 * e + 4 * hi) =
+    for (int e = 0; e < AE; e += 4)
+      *reinterpret_cast<uint2 *>(out + RB * i + NG * e + 4 * g) =
           make_uint2(M::pack(o[i][e] * f, o[i][e + 1] * f),
                      M::pack(o[i][e + 2] * f, o[i][e + 3] * f));
 }
 
-// Joins the parts of tiles that were cut.  D / 4 lanes hold a row; ALL: all of the
-// workgroup's groups of lanes share one row's parts (few rows of many parts),
-// otherwise each takes rows of its own.
-template <class T, int D, int kRows, bool ALL>
-__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, AttnPlan p) {
-  constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
-  __shared__ f32x4 acc[ALL ? 256 : 1];
+// Joins the parts of tiles that were cut.  D / 4 lanes hold a row's columns; up to 8
+// parts go to one such group, whose loads are on their way together, and more to
+// several groups, joined through LDS.  The workgroups z of a tile share its rows.
+constexpr int kJoinThreads = 512;
+template <class T, int D>
+__global__ __launch_bounds__(kJoinThreads) void attn_join_kernel(AttnArgs a, AttnPlan p, int rows) {
+  constexpr int kLanes = D / 4, kGroups = kJoinThreads / kLanes;
+  __shared__ f32x4 acc[kJoinThreads];
   __shared__ float2 ml[kGroups];
   const KvArgs &kv = a.kv;
   const int lane = threadIdx.x & 63;
   const int shares = kv.heads * p.hchunks, share = blockIdx.y;
   const AttnItem it = find_item(kv, p, a.window, blockIdx.x, true, lane);
   if (!it.live || it.parts < 2) return;
-  const SeqSpan sp = kv_span(kv, it.seq);
-  const AttnTile tl = attn_tile(sp, it.tile, p.tpt, a.window);
+  const AttnTile tl = attn_tile(it.sp, it.tile, p.tpt, a.window);
   const int group = a.heads / kv.heads;
   const int g = threadIdx.x / kLanes, col = (threadIdx.x % kLanes) * 4;
-  const int step = ALL ? gridDim.z : gridDim.z * kGroups;
-  for (int r = ALL ? blockIdx.z : blockIdx.z * kGroups + g; r < p.tpt * p.hpt; r += step) {
+  int each = 1;   // groups a row
+  while (each < kGroups && 8 * each < it.parts) each *= 2;
+  const int side = kGroups / each, mine = g % each;   // rows at a time
+  for (int r0 = blockIdx.z * side; r0 < tl.tokens * p.hpt; r0 += gridDim.z * side) {
+    const int r = r0 + g / each;
     const int tok = r / p.hpt, hh = (share % p.hchunks) * p.hpt + r % p.hpt;
-    if (tok >= tl.tokens) break;
-    if (hh >= group) continue;
-    const int h = (share / p.hchunks) * group + hh;
-    const float sink = a.sinks != nullptr ? a.sinks[h] * kLog2e : -INFINITY;
+    const bool live = tok < tl.tokens && hh < group;
     float m = kNoMax, l = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    // eight parts a step, so that their loads are on their way together
-    const int stride = ALL ? kGroups : 1;
-    for (int i0 = ALL ? g : 0; i0 < it.parts; i0 += 8 * stride) {
+    for (int i0 = mine; live && i0 < it.parts; i0 += 8 * each) {
       float2 w[8];
       f32x4 v[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const int i = min(i0 + k * stride, it.parts - 1);
-        const int64_t at = ((int64_t)(it.first + i) * shares + share) * kRows + r;
+        const int i = min(i0 + k * each, it.parts - 1);
+        const int64_t at = ((int64_t)(it.first + i) * shares + share) * rows + r;
         w[k] = p.pml[at];
         v[k] = *reinterpret_cast<const f32x4 *>(p.po + at * D + col);
-        if (i0 + k * stride >= it.parts) w[k] = make_float2(kNoMax, 0.f);
+        if (i0 + k * each >= it.parts) w[k] = make_float2(kNoMax, 0.f);
       }
       float mm = m;
 #pragma unroll
       for (int k = 0; k < 8; ++k) mm = fmaxf(mm, w[k].x);
-      float f = __builtin_amdgcn_exp2f(m - mm);
+      const float f = __builtin_amdgcn_exp2f(m - mm);
       l *= f;
       o *= f;
       m = mm;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        if (w[k].y == 0.f) continue;   // (its columns were not written)
-        f = __builtin_amdgcn_exp2f(w[k].x - m);
+        const float f = __builtin_amdgcn_exp2f(w[k].x - m);
         l = fmaf(w[k].y, f, l);
-        o += v[k] * f;
+        // (a part of no seen key wrote no columns)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = w[k].y == 0.f ? o[e] : fmaf(v[k][e], f, o[e]);
       }
     }
-    if (ALL) {
+    if (each > 1) {
       __syncthreads();
       acc[threadIdx.x] = o;
       if (col == 0) ml[g] = make_float2(m, l);
       __syncthreads();
-      if (g != 0) continue;
-      float mm = kNoMax;
-      for (int k = 0; k < kGroups; ++k) mm = fmaxf(mm, ml[k].x);
-      l = 0.f;
-      o = (f32x4){0.f, 0.f, 0.f, 0.f};
-      for (int k = 0; k < kGroups; ++k) {
-        const float f = __builtin_amdgcn_exp2f(ml[k].x - mm);
-        l = fmaf(ml[k].y, f, l);
-        o += acc[k * kLanes + threadIdx.x] * f;
+      if (mine == 0) {
+        float mm = m;
+        for (int k = 1; k < each; ++k) mm = fmaxf(mm, ml[g + k].x);
+        float f = __builtin_amdgcn_exp2f(m - mm);
+        l *= f;
+        o *= f;
+        for (int k = 1; k < each; ++k) {
+          f = __builtin_amdgcn_exp2f(ml[g + k].x - mm);
+          l = fmaf(ml[g + k].y, f, l);
+          o += acc[threadIdx.x + k * kLanes] * f;
+        }
+        m = mm;
       }
-      m = mm;
     }
-    const float mm = fmaxf(m, sink);
-    float f = __builtin_amdgcn_exp2f(m - mm);
-    l = l * f + __builtin_amdgcn_exp2f(sink - mm);
-    f = l == 0.f ? 0.f : f / l;
+    if (mine != 0 || !live) continue;
+    const int h = (share / p.hchunks) * group + hh;
+    if (a.sinks != nullptr) {
+      const float sink = a.sinks[h] * kLog2e, mm = fmaxf(m, sink);
+      const float f = __builtin_amdgcn_exp2f(m - mm);
+      l = l * f + __builtin_amdgcn_exp2f(sink - mm);
+      o *= f;
+    }
+    const float f = l == 0.f ? 0.f : 1.f / l;
     uint16_t *const out = a.out + ((int64_t)(tl.row0 + tok) * a.heads + h) * D + col;
     *reinterpret_cast<uint2 *>(out) =
-        make_uint2(Mfma32<T>::pack(o[0] * f, o[1] * f), Mfma32<T>::pack(o[2] * f, o[3] * f));
+        make_uint2(Mat<T>::pack(o[0] * f, o[1] * f), Mat<T>::pack(o[2] * f, o[3] * f));
   }
 }
 
@@ -558,68 +741,72 @@ bool attn_supported(int dim, int heads, int kv_heads) {
 namespace {
 
 // Rows of a tile: 256 (8 waves on the same keys) where a sequence brings that many
-// rows a key head on average, otherwise 32 (2 waves on keys of their own).
+// rows a key head on average, otherwise 32 or 16 (waves on keys of their own).
 struct AttnShape {
-  bool wide;
+  int rows;
   AttnPlan plan;
   int tiles;
+  bool cut;   // whether a sequence may come in parts
 };
-constexpr int kWideRows = 256, kNarrowRows = 32;
-AttnShape attn_shape(const KvArgs &kv, int heads) {
+AttnShape attn_shape(const KvArgs &kv, int heads, int window) {
   AttnShape s;
   const int group = heads / kv.heads;
-  s.wide = (int64_t)kv.total * group >= (int64_t)96 * kv.n_seqs;
-  const int rows = s.wide ? kWideRows : kNarrowRows;
-  s.plan.hpt = std::min(group, rows);
+  const int64_t mean = ((int64_t)kv.total * group + kv.n_seqs - 1) / kv.n_seqs;
+  s.rows = mean > 96 ? 256 : mean > 16 ? 32 : 16;
+  s.plan.hpt = std::min(group, s.rows);
   s.plan.hchunks = (group + s.plan.hpt - 1) / s.plan.hpt;
-  s.plan.tpt = rows / s.plan.hpt;
+  s.plan.tpt = s.rows / s.plan.hpt;
   // a tile holds a token at least
   s.tiles = (int)std::min<int64_t>(kv.total, (int64_t)kv.total / s.plan.tpt + kv.n_seqs);
-  s.plan.target = s.wide ? 512 : 1024;
-  s.plan.least = s.wide ? 512 : 256;
+  s.plan.target = s.rows == 256 ? 512 : 1024;
+  s.plan.least = s.rows == 256 ? 512 : 256;
+  SeqSpan longest = {};
+  longest.len = kv.width << kv.page_shift;
+  s.cut = span_keys(longest, window, s.plan.tpt) > s.plan.least;
   const int shares = kv.heads * s.plan.hchunks;
-  s.plan.items = s.tiles + (s.plan.target + shares - 1) / shares;
+  s.plan.items = s.tiles + s.plan.target / shares + 2;
   return s;
 }
-size_t attn_part_bytes(const KvArgs &kv, const AttnShape &s) {
-  return (size_t)s.plan.items * kv.heads * s.plan.hchunks * (s.wide ? kWideRows : kNarrowRows);
+size_t attn_part_rows(const KvArgs &kv, const AttnShape &s) {
+  return (size_t)s.plan.items * kv.heads * s.plan.hchunks * s.rows;
 }
 
 }  // namespace
 
 // Launches count threads in 32 bits.
-bool attn_fits(const KvArgs &kv, int heads) {
-  const AttnShape s = attn_shape(kv, heads);
+bool attn_fits(const KvArgs &kv, int heads, int window) {
+  const AttnShape s = attn_shape(kv, heads, window);
   const int64_t shares = (int64_t)kv.heads * s.plan.hchunks;
   return shares < 65536 && ((int64_t)s.plan.items * shares) < (1 << 23) && s.tiles < (1 << 24);
 }
 
-size_t attn_workspace(const KvArgs &kv, int heads) {
-  const AttnShape s = attn_shape(kv, heads);
-  return (attn_part_bytes(kv, s) * (kv.dim * 4 + 8) + 255) & ~(size_t)255;
+size_t attn_workspace(const KvArgs &kv, int heads, int window) {
+  const AttnShape s = attn_shape(kv, heads, window);
+  return s.cut ? (attn_part_rows(kv, s) * (kv.dim * 4 + 8) + 255) & ~(size_t)255 : 0;
+}
+
+template <class T, int D, int RB, int QW, int KW, int BK>
+static void attn_run(const AttnArgs &a, const AttnShape &sh, hipStream_t s) {
+  const int shares = a.kv.heads * sh.plan.hchunks;
+  hipLaunchKernelGGL((attn_kernel<T, D, RB, QW, KW, BK>),
+                     dim3((unsigned)(sh.plan.items * shares)), dim3(64 * QW * KW), 0, s, a,
+                     sh.plan);
+  if (!sh.cut) return;
+  // (few tiles have many parts, and then a workgroup a row; many have few)
+  const int z = std::min(sh.plan.tpt * sh.plan.hpt, std::max(1, 512 / (sh.tiles * shares)));
+  hipLaunchKernelGGL((attn_join_kernel<T, D>), dim3(sh.tiles, shares, z), dim3(kJoinThreads), 0,
+                     s, a, sh.plan, sh.rows);
 }
 
 template <class T, int D>
 static void attn_go(const AttnArgs &a, void *ws, hipStream_t s) {
-  AttnShape sh = attn_shape(a.kv, a.heads);
-  const size_t n = attn_part_bytes(a.kv, sh);
+  AttnShape sh = attn_shape(a.kv, a.heads, a.window);
   sh.plan.po = static_cast<float *>(ws);
-  sh.plan.pml = reinterpret_cast<float2 *>(sh.plan.po + n * D);
-  const int shares = a.kv.heads * sh.plan.hchunks;
-  const dim3 g((unsigned)(sh.plan.items * shares));
-  if (sh.wide) {
-    constexpr int BK = 64;
-    hipLaunchKernelGGL((attn_kernel<T, D, 8, 1, BK>), g, dim3(512), 0, s, a,
-                       sh.plan);
-    hipLaunchKernelGGL((attn_join_kernel<T, D, kWideRows, false>), dim3(sh.tiles, shares, 4),
-                       dim3(256), 0, s, a, sh.plan);
-  } else {
-    constexpr int BK = D == 128 ? 32 : 64, KW = 2;
-    hipLaunchKernelGGL((attn_kernel<T, D, 1, KW, BK>), g, dim3(64 * KW), 0, s,
-                       a, sh.plan);
-    hipLaunchKernelGGL((attn_join_kernel<T, D, kNarrowRows, true>),
-                       dim3(sh.tiles, shares, sh.plan.hpt), dim3(256), 0, s, a, sh.plan);
-  }
+  sh.plan.pml = reinterpret_cast<float2 *>(sh.plan.po + attn_part_rows(a.kv, sh) * D);
+  constexpr int KW = D == 128 ? 1 : 2;
+  if (sh.rows == 256) attn_run<T, D, 32, 8, 1, 64>(a, sh, s);
+  else if (sh.rows == 32) attn_run<T, D, 32, 1, KW, 32>(a, sh, s);
+  else attn_run<T, D, 16, 1, KW, 32>(a, sh, s);
 }
 
 void launch_attn(const AttnArgs &a, int dtype, void *ws, hipStream_t s) {

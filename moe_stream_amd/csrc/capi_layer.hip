@@ -188,10 +188,11 @@ int moe_rope_cache(const moe_kv_view *kv, const void *q, int64_t q_token, int64_
   return MOE_OK;
 }
 
-size_t moe_attn_paged_workspace(const moe_kv_view *kv, int32_t T, int32_t heads) {
+size_t moe_attn_paged_workspace(const moe_kv_view *kv, int32_t T, int32_t heads,
+                                int32_t window) {
   moe::KvArgs a;
-  if (T <= 0 || heads <= 0 || make_kv_args(kv, T, &a)) return 0;
-  return moe::attn_workspace(a, heads);
+  if (T <= 0 || heads <= 0 || window < 0 || make_kv_args(kv, T, &a) || heads % a.heads) return 0;
+  return moe::attn_workspace(a, heads, window);
 }
 
 int moe_attn_paged(const moe_kv_view *kv, const void *q, int64_t q_token, int64_t q_head,
@@ -209,13 +210,13 @@ int moe_attn_paged(const moe_kv_view *kv, const void *q, int64_t q_token, int64_
                 kv->head_dim, heads / kv->kv_heads);
   if (window < 0) return fail(MOE_ERR_INVALID, "window=%d is negative", window);
   if (T == 0) return MOE_OK;
-  if (!moe::attn_fits(a.kv, heads))
+  if (!moe::attn_fits(a.kv, heads, window))
     return fail(MOE_ERR_UNSUPPORTED, "T=%d rows of %d heads pass one launch", T, heads);
   if (!q || !out) return fail(MOE_ERR_INVALID, "NULL q/out");
   if (!aligned(q, 16) || q_token % 8 || q_head % 8 || !aligned(kv->k, 16) ||
       !aligned(kv->v, 16) || !aligned(out, 16))
     return fail(MOE_ERR_INVALID, "q's rows, the pages and out must be 16-byte aligned");
-  const size_t need = moe::attn_workspace(a.kv, heads);
+  const size_t need = moe::attn_workspace(a.kv, heads, window);
   if (need && (!workspace || !aligned(workspace, 256)))
     return fail(MOE_ERR_INVALID, "workspace NULL or not 256-byte aligned");
   if (workspace_bytes < need)

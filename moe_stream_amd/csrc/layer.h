@@ -17,6 +17,10 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
+// s_waitcnt's argument for "at most n vector memory loads are under way", the other
+// counts as they are: what a barrier needs before it where loads go straight to LDS.
+constexpr int loads_left(int n) { return 0x0f70 | (n & 15) | (n >> 4) << 14; }
+
 // The 16-bit types: conversions round to nearest even, NaN stays NaN.
 struct Bf16 {
   static constexpr int kType = MOE_DTYPE_BF16;
@@ -192,8 +196,8 @@ struct AttnArgs {
   float scale;
 };
 bool attn_supported(int dim, int heads, int kv_heads);
-bool attn_fits(const KvArgs &kv, int heads);
-size_t attn_workspace(const KvArgs &kv, int heads);
+bool attn_fits(const KvArgs &kv, int heads, int window);
+size_t attn_workspace(const KvArgs &kv, int heads, int window);
 void launch_attn(const AttnArgs &a, int dtype, void *ws, hipStream_t s);
 
 // --- 8-bit product (linear_fp8.hip) -----------------------------------------------

@@ -11,6 +11,7 @@
 // the 16-byte pieces g and g + 4 of its row (g = lane / 16), so that a load of 64
 // lanes covers 64 bytes in a row of each of 16 rows.
 #include <algorithm>
+#include <type_traits>
 
 #include "layer.h"
 
@@ -78,60 +79,81 @@ __global__ __launch_bounds__(64 * kThinWaves) void linear_thin_kernel(LinearArgs
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
   const u32x4_t none = {0, 0, 0, 0};
-#pragma unroll 2
-  for (int b = wave; b < blocks; b += kThinWaves) {
-    const int k0 = b * kFp8Block + 16 * g, k1 = k0 + 64;
-    const bool in0 = k0 < a.K, in1 = k1 < a.K;   // (K is whole pieces)
-    i32x8 wf[NT], xf[TT];
-    float sc[TT];
+  // One block's operands as they come: 16 bytes a piece, of x in 16 bits two for one.
+  struct Operands {
+    u32x4_t w[NT][2], x[TT][kX16 ? 4 : 2];
+    float xs[TT], ws;
+  };
+  auto load = [&](Operands &o, int b) __attribute__((always_inline)) {
+    const int k[2] = {b * kFp8Block + 16 * g, b * kFp8Block + 16 * g + 64};
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
-      wf[j] = pieces(in0 ? __builtin_nontemporal_load(reinterpret_cast<const u32x4_t *>(w[j] + k0)) : none,
-                     in1 ? __builtin_nontemporal_load(reinterpret_cast<const u32x4_t *>(w[j] + k1)) : none);
+    for (int p = 0; p < 2; ++p) {
+      const bool in = k[p] < a.K;   // (K is whole pieces)
 #pragma unroll
-    for (int i = 0; i < TT; ++i) {
-      if constexpr (kX16) {
-        const uint16_t *x = reinterpret_cast<const uint16_t *>(a.x) + t[i] * a.x_stride;
-        float v[4][8];
-        load8<XT>(x + k0, in0 ? 8 : 0, v[0]);
-        load8<XT>(x + k0 + 8, in0 ? 8 : 0, v[1]);
-        load8<XT>(x + k1, in1 ? 8 : 0, v[2]);
-        load8<XT>(x + k1 + 8, in1 ? 8 : 0, v[3]);
-        uint32_t m = __float_as_uint(kFp8Least);
+      for (int j = 0; j < NT; ++j)
+        o.w[j][p] =
+            in ? __builtin_nontemporal_load(reinterpret_cast<const u32x4_t *>(w[j] + k[p])) : none;
 #pragma unroll
-        for (int e = 0; e < 32; ++e) m = max(m, __float_as_uint(v[e / 8][e % 8]) & 0x7fffffffu);
-        m = max(m, (uint32_t)__shfl_xor((int)m, 16));
-        m = max(m, (uint32_t)__shfl_xor((int)m, 32));
-        u32x4_t lo, hi;
+      for (int i = 0; i < TT; ++i) {
+        if constexpr (kX16) {
+          const uint16_t *x = reinterpret_cast<const uint16_t *>(a.x) + t[i] * a.x_stride + k[p];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const uint2 c = to_fp8(v[e], m), d = to_fp8(v[2 + e], m);
-          lo[2 * e] = c.x;
-          lo[2 * e + 1] = c.y;
-          hi[2 * e] = d.x;
-          hi[2 * e + 1] = d.y;
+          for (int e = 0; e < 2; ++e)
+            o.x[i][2 * p + e] = in ? *reinterpret_cast<const u32x4_any *>(x + 8 * e) : none;
+        } else {
+          const uint8_t *x = a.x + t[i] * a.x_stride + k[p];
+          o.x[i][p] = in ? *reinterpret_cast<const u32x4_t *>(x) : none;
         }
-        xf[i] = pieces(lo, hi);
-        sc[i] = fp8_scale(m);
-      } else {
-        const uint8_t *x = a.x + t[i] * a.x_stride;
-        xf[i] = pieces(in0 ? *reinterpret_cast<const u32x4_t *>(x + k0) : none,
-                       in1 ? *reinterpret_cast<const u32x4_t *>(x + k1) : none);
-        sc[i] = a.xs[(int64_t)t[i] * blocks + b];
       }
     }
     // (16 NT outputs lie in one block of 128)
-    const float ws = a.ws[(int64_t)(n0 / kFp8Block) * blocks + b];
+    o.ws = a.ws[(int64_t)(n0 / kFp8Block) * blocks + b];
+    if constexpr (!kX16) {
+#pragma unroll
+      for (int i = 0; i < TT; ++i) o.xs[i] = a.xs[(int64_t)t[i] * blocks + b];
+    }
+  };
+  auto multiply = [&](const Operands &o) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < TT; ++i) {
-      const float f = sc[i] * ws;
+      i32x8 xf;
+      float xs = o.xs[i];
+      if constexpr (kX16) {
+        float v[4][8];
+        uint32_t m = __float_as_uint(kFp8Least);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const uint32_t pair = o.x[i][e / 8][e % 8 / 2];
+          v[e / 8][e % 8] = XT::load(e & 1 ? pair >> 16 : pair & 0xffffu);
+          m = max(m, __float_as_uint(v[e / 8][e % 8]) & 0x7fffffffu);
+        }
+        m = max(m, (uint32_t)__shfl_xor((int)m, 16));
+        m = max(m, (uint32_t)__shfl_xor((int)m, 32));
+        u32x4_t c[2];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint2 q = to_fp8(v[e], m);
+          c[e / 2][2 * (e & 1)] = q.x;
+          c[e / 2][2 * (e & 1) + 1] = q.y;
+        }
+        xf = pieces(c[0], c[1]);
+        xs = fp8_scale(m);
+      } else {
+        xf = pieces(o.x[i][0], o.x[i][1]);
+      }
+      const float f = xs * o.ws;
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        const f32x4 p = mfma_e4m3(wf[j], xf[i]);
+        const f32x4 p = mfma_e4m3(pieces(o.w[j][0], o.w[j][1]), xf);
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(p[e], f, acc[i][j][e]);
       }
     }
+  };
+  for (int b = wave; b < blocks; b += kThinWaves) {
+    Operands o;
+    load(o, b);
+    multiply(o);
   }
 #pragma unroll
   for (int i = 0; i < TT; ++i)
@@ -148,109 +170,192 @@ __global__ __launch_bounds__(64 * kThinWaves) void linear_thin_kernel(LinearArgs
 }
 
 // ---------------------------------------------------------------------------
-// Many rows: a workgroup's 4 waves take a tile of 2 * 16 R rows by as many outputs,
-// each a quarter of it.  The tile's block of 128 columns of x and of w goes straight
-// to LDS a block ahead, 16-byte pieces permuted within a row (two rows of 128 bytes
-// span the banks) so that 16 rows' reads of a piece meet no conflict.  The scales of
-// the lane's rows are a block ahead in registers.
+// Many rows: a workgroup's WT x WN waves take a tile of 16 RT WT rows by 16 RN WN
+// outputs, each wave 16 RT x 16 RN of it.  The tile's block of 128 columns of x and of w
+// goes straight to LDS a block ahead, 16-byte pieces permuted within a row (two rows of
+// 128 bytes span the banks) so that 16 rows' reads of a piece meet no conflict.  The
+// scales of the lane's rows are a block ahead in registers.
 // ---------------------------------------------------------------------------
 typedef __attribute__((address_space(3))) void lds_void;
 typedef const __attribute__((address_space(1))) void global_void;
 
-template <class T, int R>
-__global__ __launch_bounds__(256, 2) void linear_tile_kernel(LinearArgs a, int t_tiles) {
-  constexpr int kRows = 32 * R;                // of x, and of w
-  constexpr int kBytes = kRows * kFp8Block;
-  constexpr int kLoads = kRows / 8 / 4;        // a wave's loads of x, and of w: 8 rows each
-  __shared__ __align__(1024) char lds[2][2][kBytes];
+template <class T, int RT, int RN, int WT, int WN>
+__global__ __launch_bounds__(64 * WT * WN, 2) void linear_tile_kernel(LinearArgs a, int t_tiles) {
+  constexpr int W = WT * WN;
+  constexpr int kT = 16 * RT * WT, kN = 16 * RN * WN;
+  constexpr int kLoadsX = kT / 8 / W, kLoadsW = kN / 8 / W;   // a wave's, 8 rows each
+  // (an array of its own for each tile: loads to one are under way while another is
+  // read, which the compiler waits for unless it tells them apart)
+  __shared__ __align__(1024) char lds_x0[kT * kFp8Block], lds_x1[kT * kFp8Block];
+  __shared__ __align__(1024) char lds_w0[kN * kFp8Block], lds_w1[kN * kFp8Block];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // neighbouring workgroups go to the 8 dies in turn: each die takes a run of tiles,
-  // all row tiles of an output tile before the next, so its weights stay in its cache
+  // Neighbouring workgroups go to the 8 dies in turn: each die takes a run of tiles, and
+  // within bands of 8 row tiles all of an output tile before the next, so that the tiles
+  // a die has at once read few rows of x and of w.
   const int total = gridDim.x, each = total / 8, more = total % 8;
   const int die = blockIdx.x % 8;
   const int tile = die * each + min(die, more) + blockIdx.x / 8;
-  const int t0 = (tile % t_tiles) * kRows, n0 = (tile / t_tiles) * kRows;
+  const int n_tiles = total / t_tiles, band = tile / (8 * n_tiles), in = tile % (8 * n_tiles);
+  const int wide = min(8, t_tiles - band * 8);
+  const int t0 = (band * 8 + in % wide) * kT, n0 = (in / wide) * kN;
   const int blocks = (a.K + kFp8Block - 1) / kFp8Block;
   const int last = a.K / 16 - 1;               // the last piece of a row
 
+  // Rows past the end are the last one again, and not stored.
   const int sub = lane / 8, piece = lane % 8;
-  auto fetch = [&](int b, int buf) {
+  uint32_t xo[kLoadsX], wo[kLoadsW];
+  const uint8_t *const x0 = a.x + min(t0, a.T - 1) * a.x_stride;
+  const uint8_t *const w0 = a.w + (int64_t)min(n0, a.N - 1) * a.K;
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int row = (i * 4 + wave) * 8 + sub;
-      // (a piece past K is the row's last one again; x's are zeroed where they are used)
-      const int64_t k = 16 * (int64_t)min(b * 8 + (piece ^ ((row >> 1) & 7)), last);
-      const uint8_t *gx = a.x + min(t0 + row, a.T - 1) * a.x_stride + k;
-      const uint8_t *gw = a.w + (int64_t)min(n0 + row, a.N - 1) * a.K + k;
-      __builtin_amdgcn_global_load_lds((global_void *)gx,
-                                       (lds_void *)(&lds[buf][0][(i * 4 + wave) * 1024]), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((global_void *)gw,
-                                       (lds_void *)(&lds[buf][1][(i * 4 + wave) * 1024]), 16, 0, 0);
-    }
+  for (int i = 0; i < kLoadsX; ++i)
+    xo[i] = (uint32_t)(min((i * W + wave) * 8 + sub, a.T - 1 - t0) * a.x_stride);
+#pragma unroll
+  for (int i = 0; i < kLoadsW; ++i)
+    wo[i] = (uint32_t)(min((i * W + wave) * 8 + sub, a.N - 1 - n0) * a.K);
+  // The k-th load of block b: rows of x, then of w.  (A piece past K is the row's last
+  // one again; x's are zeroed where they are used.)
+  const int pc = piece ^ ((wave * 4 + sub / 2) & 7);
+  auto fetch = [&](int b, int k, char *to_x, char *to_w) __attribute__((always_inline)) {
+    const uint32_t at = 16 * min(b * 8 + pc, last);
+    if (k < kLoadsX)
+      __builtin_amdgcn_global_load_lds((global_void *)(x0 + (xo[k % kLoadsX] + at)),
+                                       (lds_void *)(to_x + (k * W + wave) * 1024), 16, 0, 0);
+    else
+      __builtin_amdgcn_global_load_lds((global_void *)(w0 + (wo[(k - kLoadsX) % kLoadsW] + at)),
+                                       (lds_void *)(to_w + ((k - kLoadsX) * W + wave) * 1024), 16,
+                                       0, 0);
   };
   const int row = lane & 15, g = lane >> 4;
-  const int tw = (wave & 1) * 16 * R, nw = (wave >> 1) * 16 * R;   // the wave's quarter
-  const float *xs[R];
+  const int tw = (wave % WT) * 16 * RT, nw = (wave / WT) * 16 * RN;   // the wave's share
+  const float *xs[RT];
 #pragma unroll
-  for (int i = 0; i < R; ++i) xs[i] = a.xs + (int64_t)min(t0 + tw + 16 * i + row, a.T - 1) * blocks;
+  for (int i = 0; i < RT; ++i)
+    xs[i] = a.xs + (int64_t)min(t0 + tw + 16 * i + row, a.T - 1) * blocks;
+  // (16 RN outputs lie in one block of 128)
   const float *ws = a.ws + (int64_t)(min(n0 + nw, a.N - 1) / kFp8Block) * blocks;
-  float sc[R], sw = ws[0];
+  float sc[RT], sw = ws[0];
 #pragma unroll
-  for (int i = 0; i < R; ++i) sc[i] = xs[i][0];
-  f32x4 acc[R][R];
+  for (int i = 0; i < RT; ++i) sc[i] = xs[i][0];
+  f32x4 acc[RT][RN];
 #pragma unroll
-  for (int i = 0; i < R; ++i)
+  for (int i = 0; i < RT; ++i)
 #pragma unroll
-    for (int j = 0; j < R; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < RN; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
 
-  auto frag = [&](const char *tile_lds, int r) {
-    const int f = (r >> 1) & 7;
-    const char *p = tile_lds + r * kFp8Block;
-    return pieces(*reinterpret_cast<const u32x4_t *>(p + ((g ^ f) * 16)),
-                  *reinterpret_cast<const u32x4_t *>(p + (((g + 4) ^ f) * 16)));
+  // Where a lane reads in a tile, but for the block of 16 rows: one value each, so that
+  // the compiler keeps sight of which array is read.
+  const int f = (row >> 1) & 7;
+  int x_at = (tw + row) * kFp8Block + (g ^ f) * 16, w_at = (nw + row) * kFp8Block + (g ^ f) * 16;
+  asm("" : "+v"(x_at), "+v"(w_at));
+  auto frag = [&](const char *tile, int at, int r) __attribute__((always_inline)) {
+    return pieces(*reinterpret_cast<const u32x4_t *>(tile + at + r * 16 * kFp8Block),
+                  *reinterpret_cast<const u32x4_t *>(tile + (at ^ 64) + r * 16 * kFp8Block));
   };
-  fetch(0, 0);
-  for (int b = 0; b < blocks; ++b) {
+  auto block = [&](int b, const char *in_x, const char *in_w, char *to_x, char *to_w)
+      __attribute__((always_inline)) {
+    issue_order_fence();
+    __builtin_amdgcn_s_waitcnt(loads_left(0));
     __syncthreads();   // block b has landed, and block b - 1 is read
-    float f[R];
+    issue_order_fence();
+    float f[RT];
 #pragma unroll
-    for (int i = 0; i < R; ++i) f[i] = sc[i] * sw;
-    if (b + 1 < blocks) {
-      fetch(b + 1, (b + 1) & 1);
+    for (int i = 0; i < RT; ++i) f[i] = sc[i] * sw;
+    const bool end = b + 1 == blocks;
+    const int next = min(b + 1, blocks - 1);   // (the last block again, not used)
 #pragma unroll
-      for (int i = 0; i < R; ++i) sc[i] = xs[i][b + 1];
-      sw = ws[b + 1];
-    }
-    i32x8 xf[R];
+    for (int i = 0; i < RT; ++i) sc[i] = xs[i][next];
+    sw = ws[next];
+    constexpr int kAhead = 3;   // outputs' operands under way
+    i32x8 xf[RT], wf[kAhead];
+    wf[0] = frag(in_w, w_at, 0);
 #pragma unroll
-    for (int i = 0; i < R; ++i) xf[i] = frag(lds[b & 1][0], tw + 16 * i + row);
-    if (b + 1 == blocks && a.K % kFp8Block) {
+    for (int i = 0; i < RT; ++i) xf[i] = frag(in_x, x_at, i);
+#pragma unroll
+    for (int j = 1; j < kAhead - 1 && j < RN; ++j) wf[j] = frag(in_w, w_at, j);
+    if (end && a.K % kFp8Block) {
       const int left = (a.K % kFp8Block) / 16;
 #pragma unroll
-      for (int i = 0; i < R; ++i)
+      for (int i = 0; i < RT; ++i)
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           if ((e < 4 ? g : g + 4) >= left) xf[i][e] = 0;
     }
+    // A product is folded while the two after it run; the next block's loads and the
+    // next outputs' operand go between.
+    constexpr int kLag = 2, kMul = RT * RN, kLoads = kLoadsX + kLoadsW;
+    constexpr int kEach = (2 * kLoads + kMul - 1) / kMul;   // (gone by the half)
+    f32x4 p[kLag + 1];
 #pragma unroll
-    for (int j = 0; j < R; ++j) {
-      const i32x8 wf = frag(lds[b & 1][1], nw + 16 * j + row);
+    for (int u = 0; u < kMul + kLag; ++u) {
+      const int j = u / RT, i = u % RT;
+      if (u < kMul) {
+        if (i == 0 && j + kAhead - 1 < RN)
+          wf[(j + kAhead - 1) % kAhead] = frag(in_w, w_at, j + kAhead - 1);
+        p[u % (kLag + 1)] = mfma_e4m3(wf[j % kAhead], xf[i]);
 #pragma unroll
-      for (int i = 0; i < R; ++i) {
-        const f32x4 p = mfma_e4m3(wf, xf[i]);
+        for (int k = kEach * u; k < kEach * (u + 1) && k < kLoads; ++k) fetch(next, k, to_x, to_w);
+      }
+      if (u >= kLag) {
+        const int v = u - kLag, vj = v / RT, vi = v % RT;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(p[e], f[i], acc[i][j][e]);
+        for (int e = 0; e < 4; ++e) {
+          acc[vi][vj][e] = fmaf(p[v % (kLag + 1)][e], f[vi], acc[vi][vj][e]);
+          asm volatile("" : "+v"(acc[vi][vj][e]));   // (here, between the products)
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+#pragma unroll
+  for (int k = 0; k < kLoadsX + kLoadsW; ++k) fetch(0, k, lds_x0, lds_w0);
+  for (int b = 0; b < blocks; b += 2) {
+    block(b, lds_x0, lds_w0, lds_x1, lds_w1);
+    if (b + 1 < blocks) block(b + 1, lds_x1, lds_w1, lds_x0, lds_w0);
+  }
+  // Each wave turns its share round through LDS, a block of 16 rows at a time, so that a
+  // row's outputs leave in whole pieces of 16 bytes.
+  issue_order_fence();
+  __builtin_amdgcn_s_waitcnt(loads_left(0));
+  __syncthreads();
+  constexpr int kCols = 16 * RN, kPad = kCols + 8;   // (16 bytes more a row: other banks)
+  static_assert(W / 2 * 16 * kPad * 2 <= kT * kFp8Block, "the waves' boxes fit two tiles of x");
+  uint16_t *const box =
+      reinterpret_cast<uint16_t *>(wave < W / 2 ? lds_x0 : lds_x1) + wave % (W / 2) * 16 * kPad;
+  float bias[RN][4];
+#pragma unroll
+  for (int j = 0; j < RN; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int n = n0 + nw + 16 * j + 4 * g + e;
+      bias[j][e] = a.bias != nullptr ? T::load(a.bias[min(n, a.N - 1)]) : 0.f;
+    }
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+#pragma unroll
+    for (int j = 0; j < RN; ++j) {
+      const f32x4 v = acc[i][j];
+      const uint32_t lo = T::store(v[0] + bias[j][0]) | (T::store(v[1] + bias[j][1]) << 16);
+      const uint32_t hi = T::store(v[2] + bias[j][2]) | (T::store(v[3] + bias[j][3]) << 16);
+      *reinterpret_cast<uint2 *>(box + row * kPad + 16 * j + 4 * g) = make_uint2(lo, hi);
+    }
+    issue_order_fence();   // (a wave's own LDS operations stay in order)
+    constexpr int kEach = kCols / 8;   // pieces a row
+#pragma unroll
+    for (int q = 0; q < 16 * kEach / 64; ++q) {
+      const int r = (q * 64 + lane) / kEach, c = (q * 64 + lane) % kEach * 8;
+      const u32x4_t v = *reinterpret_cast<const u32x4_t *>(box + r * kPad + c);
+      const int t = t0 + tw + 16 * i + r, n = n0 + nw + c;
+      uint16_t *const y = a.y + (int64_t)t * a.N + n;
+      if (t < a.T && n + 8 <= a.N) {
+        *reinterpret_cast<u32x4_any *>(y) = v;
+      } else if (t < a.T) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (n + e < a.N) y[e] = (uint16_t)(v[e / 2] >> (16 * (e & 1)));
       }
     }
-  }
-#pragma unroll
-  for (int i = 0; i < R; ++i) {
-    const int t = t0 + tw + 16 * i + row;
-    if (t < a.T) {
-#pragma unroll
-      for (int j = 0; j < R; ++j) store_outputs<T>(a, t, n0 + nw + 16 * j + 4 * g, acc[i][j]);
-    }
+    issue_order_fence();
   }
 }
 
@@ -277,6 +382,7 @@ static void linear_go(const LinearArgs &a, int x_dtype, hipStream_t s) {
     else if (x_dtype == MOE_DTYPE_F16) thin_go<T, F16, 1>(a, s);
     else if (a.T <= 16) thin_go<T, uint8_t, 1>(a, s);
     else if (a.T <= 32) thin_go<T, uint8_t, 2>(a, s);
+    else if (a.T <= 48) thin_go<T, uint8_t, 3>(a, s);
     else thin_go<T, uint8_t, 4>(a, s);
     return;
   }
@@ -285,13 +391,13 @@ static void linear_go(const LinearArgs &a, int x_dtype, hipStream_t s) {
     return *t_tiles * ((a.N + rows - 1) / rows);
   };
   int tt;
-  const int n = tiles(128, &tt);
-  if (n >= 256) {
-    hipLaunchKernelGGL((linear_tile_kernel<T, 4>), dim3(n), dim3(256), 0, s, a, tt);
-  } else {
-    const int m = tiles(64, &tt);
-    hipLaunchKernelGGL((linear_tile_kernel<T, 2>), dim3(m), dim3(256), 0, s, a, tt);
-  }
+  if (const int n = tiles(256, &tt); n >= 256)
+    hipLaunchKernelGGL((linear_tile_kernel<T, 4, 8, 4, 2>), dim3(n), dim3(512), 0, s, a, tt);
+  else if (const int n = tiles(128, &tt); n >= 256)
+    hipLaunchKernelGGL((linear_tile_kernel<T, 4, 4, 2, 2>), dim3(n), dim3(256), 0, s, a, tt);
+  else
+    hipLaunchKernelGGL((linear_tile_kernel<T, 2, 2, 2, 2>), dim3(tiles(64, &tt)), dim3(256), 0, s,
+                       a, tt);
 }
 
 void launch_linear(const LinearArgs &a, int x_dtype, int out_dtype, hipStream_t s) {

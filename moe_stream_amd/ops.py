@@ -620,7 +620,7 @@ def attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     else:
         _req(out, q.dtype, "out", T * H * D, dev)
     L = _lib.lib()
-    need = L.moe_attn_paged_workspace(C.byref(kv), T, H)
+    need = L.moe_attn_paged_workspace(C.byref(kv), T, H, window)
     ws = workspace
     if ws is None and need:
         ws = _WS.get("attn_paged", need, dev, handle, side=side)

@@ -98,7 +98,7 @@ def test_kv_view_refusals(bad, text):
     L, v = _lib.lib(), _view(**bad)
     _refused(_rope(v), text)
     _refused(_attn(v), text)
-    assert L.moe_attn_paged_workspace(C.byref(v), 3, 8) == 0
+    assert L.moe_attn_paged_workspace(C.byref(v), 3, 8, 0) == 0
 
 
 def _rope(v, q=FAKE, T=3, H=8, f=FAKE, rot=64, eps=1e-6, out=FAKE):
@@ -141,7 +141,7 @@ def test_attn_refusals():
     _refused(_attn(v, qh=65), "aligned")
     _refused(_attn(_view(k=FAKE + 2)), "aligned")
     _refused(_attn(v, out=FAKE + 4), "aligned")
-    need = _lib.lib().moe_attn_paged_workspace(C.byref(v), 3, 8)
+    need = _lib.lib().moe_attn_paged_workspace(C.byref(v), 3, 8, 0)
     if need:
         _refused(_attn(v, work=None), "workspace")
         _refused(_attn(v, n=need - 1), "workspace")
