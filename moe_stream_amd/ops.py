@@ -6,7 +6,6 @@ host, then launches on the current stream (or `stream`).
 from __future__ import annotations
 
 import ctypes as C
-import functools
 import math
 import threading
 from collections import OrderedDict
@@ -311,6 +310,8 @@ def check_device_error(stream=None):
 _DT16 = {torch.bfloat16: _lib.MOE_DTYPE_BF16, torch.float16: _lib.MOE_DTYPE_F16}
 
 
+# These calls take a few microseconds on the GPU for single tokens, so their checks are
+# made in one expression where all is well, and named one by one where it is not.
 def _dt16(t, name) -> int:
     d = _DT16.get(t.dtype)
     if d is None:
@@ -320,39 +321,53 @@ def _dt16(t, name) -> int:
     return d
 
 
-def _rows(t, name, dtype, shape, device):
+def _flat(t, dtype, name, numel, dev: int):
+    """_req with a device index."""
+    if (t.dtype is not dtype or t.numel() != numel or t.get_device() != dev
+            or not t.is_contiguous()):
+        _req(t, dtype, name, numel, torch.device("cuda", dev))
+
+
+def _rows(t, name, dtype, shape, dev: int):
     """t of this type, shape and device whose last dim is contiguous; its strides."""
+    st = t.stride()
+    if (t.dtype is dtype and t.shape == shape and t.get_device() == dev
+            and (st[-1] == 1 or shape[-1] == 1)):
+        return st
     if t.dtype != dtype:
         raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
     if t.shape != shape:
         raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
-    if t.device != device:
-        raise ValueError(f"{name}: on {t.device}, expected {device}")
-    st = t.stride()
-    if st[-1] != 1 and shape[-1] > 1:
-        raise ValueError(f"{name}: the last dim must be contiguous")
-    return st
+    if t.get_device() != dev:
+        raise ValueError(f"{name}: on {t.device}, expected cuda:{dev}")
+    raise ValueError(f"{name}: the last dim must be contiguous")
 
 
-def _on_device(f):
-    """Runs an operator with its first argument's device current, so that its stream
-    and workspace are that device's."""
-    @functools.wraps(f)
-    def call(first, *args, **kw):
-        if first.is_cuda and first.device.index != torch.cuda.current_device():
-            with torch.cuda.device(first.device):
-                return f(first, *args, **kw)
-        return f(first, *args, **kw)
-    return call
-
-
-def _stream_of(stream, device):
-    if stream is not None and getattr(stream, "device", device) != device:
+def _on(stream, dev: int):
+    """(the stream where it is another than the current one, the handle) for a call on
+    device index `dev`, which is the current one."""
+    if stream is None:
+        return None, torch._C._cuda_getCurrentRawStream(dev)
+    device = torch.device("cuda", dev)
+    if getattr(stream, "device", device) != device:
         raise ValueError(f"stream: on {stream.device}, expected {device}")
-    return _side(stream, device), _lib.stream_ptr(stream)
+    return _side(stream, device), int(stream.cuda_stream)
 
 
-@_on_device
+def _new(like, shape, dtype, side):
+    if side is not None:
+        return _empty(shape, dtype, like.device, side)
+    if dtype is like.dtype and shape == like.shape and like.is_contiguous():
+        return torch.empty_like(like)   # (a third quicker)
+    return torch.empty(shape, dtype=dtype, device=like.device)
+
+
+def _elsewhere(f, dev: int, *args, **kw):
+    """f with device index `dev` current, so that its stream and workspace are its."""
+    with torch.cuda.device(dev):
+        return f(*args, **kw)
+
+
 def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None,
                  eps: float = 1e-6, fp8: bool = False, out: torch.Tensor | None = None,
                  scales: torch.Tensor | None = None, summed: torch.Tensor | None = None,
@@ -367,49 +382,58 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor |
     linear_fp8 reads.  out, scales and summed are written where given (out and summed
     may be x or residual themselves)."""
     dt = _dt16(x, "x")
+    dev = x.get_device()
+    if dev != torch._C._cuda_getDevice():
+        return _elsewhere(add_rms_norm, dev, x, weight, residual, eps, fp8, out, scales, summed,
+                          stream)
     shape = x.shape
-    if x.dim() == 1:
+    if len(shape) == 1:
         x = x.view(1, -1)
         residual = residual.view(1, -1) if residual is not None else None
-    if x.dim() != 2 or x.shape[1] == 0:
+    elif len(shape) != 2:
         raise ValueError(f"x: expected [T, D], got {tuple(shape)}")
-    T, D = x.shape
-    dev = x.device
-    xs = _rows(x, "x", x.dtype, x.shape, dev)[0]
-    rs = _rows(residual, "residual", x.dtype, x.shape, dev)[0] if residual is not None else D
-    _req(weight, x.dtype, "weight", D, dev)
-    if summed is not None and residual is None:
+    T, D = rows = x.shape
+    dtype = x.dtype
+    xs = _rows(x, "x", dtype, rows, dev)[0]
+    _flat(weight, dtype, "weight", D, dev)
+    rp = rs = hp = h = None
+    side, handle = _on(stream, dev)
+    if residual is not None:
+        rs = _rows(residual, "residual", dtype, rows, dev)[0] if T > 1 else D
+        rp = residual.data_ptr()
+        if summed is None:
+            h = _new(x, shape, dtype, side)
+        else:
+            h = summed
+            _flat(h, dtype, "summed", T * D, dev)
+        hp = h.data_ptr()
+    elif summed is not None:
         raise ValueError("summed given without residual")
-    if scales is not None and not fp8:
-        raise ValueError("scales given without fp8")
-    side, handle = _stream_of(stream, dev)
-    ydt = torch.float8_e4m3fn if fp8 else x.dtype
-    if out is None:
-        out = _empty(shape, ydt, dev, side)
     else:
-        _req(out, ydt, "out", T * D, dev)
-    if fp8:
-        nb = -(-D // 128)
-        if scales is None:
-            scales = _empty((T, nb) if len(shape) == 2 else (nb,), torch.float32, dev, side)
-        else:
-            _req(scales, torch.float32, "scales", T * nb, dev)
-    if residual is None:
         h = x.view(shape)
+    ydt = torch.float8_e4m3fn if fp8 else dtype
+    if out is None:
+        out = _new(x, shape, ydt, side)
     else:
-        h = summed
-        if h is None:
-            h = _empty(shape, x.dtype, dev, side)
-        else:
-            _req(h, x.dtype, "summed", T * D, dev)
+        _flat(out, ydt, "out", T * D, dev)
+    if not fp8:
+        if scales is not None:
+            raise ValueError("scales given without fp8")
+        _lib.check(_lib.lib().moe_add_rms_norm(
+            x.data_ptr(), xs if T > 1 else D, rp, rs or D, weight.data_ptr(), dt, T, D, eps,
+            out.data_ptr(), None, None, hp, handle))
+        return out, h
+    nb = -(-D // 128)
+    if scales is None:
+        scales = _new(x, (T, nb) if len(shape) == 2 else (nb,), torch.float32, side)
+    else:
+        _flat(scales, torch.float32, "scales", T * nb, dev)
     _lib.check(_lib.lib().moe_add_rms_norm(
-        x.data_ptr(), xs if T > 1 else D, _p(residual), rs if T > 1 else D, weight.data_ptr(), dt,
-        T, D, eps, None if fp8 else out.data_ptr(), out.data_ptr() if fp8 else None, _p(scales),
-        None if residual is None else h.data_ptr(), handle))
-    return (out, scales, h) if fp8 else (out, h)
+        x.data_ptr(), xs if T > 1 else D, rp, rs or D, weight.data_ptr(), dt, T, D, eps,
+        None, out.data_ptr(), scales.data_ptr(), hp, handle))
+    return out, scales, h
 
 
-@_on_device
 def linear_fp8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor,
                x_scales: torch.Tensor | None = None, bias: torch.Tensor | None = None,
                dtype: torch.dtype | None = None, out: torch.Tensor | None = None,
@@ -421,54 +445,57 @@ def linear_fp8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor,
     with w_scales fp32 [ceil(N / 128), ceil(K / 128)]; bias [N] of the output's type:
     `dtype` (bf16 or fp16), else out's, else x's where it has 16 bits, else bf16.
     K is a multiple of 16.  Returns y [T, N] ([N] for x [K])."""
+    x8 = x.dtype is torch.float8_e4m3fn
+    if not x8:
+        dt = _dt16(x, "x")
+        if x_scales is not None:
+            raise ValueError("x_scales given with a 16-bit x")
+    elif not x.is_cuda:
+        raise TypeError("x: must be a device tensor")
+    elif x_scales is None:
+        raise ValueError("an 8-bit x needs x_scales")
+    else:
+        dt = _lib.MOE_DTYPE_E4M3
+    dev = x.get_device()
+    if dev != torch._C._cuda_getDevice():
+        return _elsewhere(linear_fp8, dev, x, w, w_scales, x_scales, bias, dtype, out, stream,
+                          workspace)
     shape = x.shape
-    if x.dim() == 1:
+    if len(shape) == 1:
         x = x.view(1, -1)
-        x_scales = x_scales.view(1, -1) if x_scales is not None else None
     if x.dim() != 2 or w.dim() != 2:
         raise ValueError(f"expected x [T, K] and w [N, K], got {tuple(shape)}, {tuple(w.shape)}")
     T, K = x.shape
     N = w.shape[0]
-    dev = x.device
-    x8 = x.dtype == torch.float8_e4m3fn
-    if x8:
-        if not x.is_cuda:
-            raise TypeError("x: must be a device tensor")
-        if x_scales is None:
-            raise ValueError("an 8-bit x needs x_scales")
-        dt = _lib.MOE_DTYPE_E4M3
-        nb = -(-K // 128)
-        _req(x_scales, torch.float32, "x_scales", T * nb, dev)
-    else:
-        dt = _dt16(x, "x")
-        if x_scales is not None:
-            raise ValueError("x_scales given with a 16-bit x")
+    nb = -(-K // 128)
     if w.shape[1] != K:
         raise ValueError(f"x has {K} columns, w {w.shape[1]}")
     xs = _rows(x, "x", x.dtype, x.shape, dev)[0]
-    _req(w, torch.float8_e4m3fn, "w", N * K, dev)
-    _req(w_scales, torch.float32, "w_scales", -(-N // 128) * -(-K // 128), dev)
+    _flat(w, torch.float8_e4m3fn, "w", N * K, dev)
+    _flat(w_scales, torch.float32, "w_scales", -(-N // 128) * nb, dev)
+    if x8:
+        _flat(x_scales, torch.float32, "x_scales", T * nb, dev)
     if dtype is None:
         dtype = out.dtype if out is not None else torch.bfloat16 if x8 else x.dtype
     odt = _DT16.get(dtype)
     if odt is None:
         raise TypeError(f"dtype: expected bfloat16 or float16, got {dtype}")
     if bias is not None:
-        _req(bias, dtype, "bias", N, dev)
-    side, handle = _stream_of(stream, dev)
+        _flat(bias, dtype, "bias", N, dev)
+    side, handle = _on(stream, dev)
     if out is None:
-        out = _empty((T, N) if len(shape) == 2 else (N,), dtype, dev, side)
+        out = _new(x, (T, N) if len(shape) == 2 else (N,), dtype, side)
     else:
-        _req(out, dtype, "out", T * N, dev)
+        _flat(out, dtype, "out", T * N, dev)
     L = _lib.lib()
-    need = L.moe_linear_fp8_workspace(T, K, N, dt)
     ws = workspace
-    if ws is None and need:
-        ws = _WS.get("linear_fp8", need, dev, handle, side=side)
+    if ws is None and not x8:
+        need = L.moe_linear_fp8_workspace(T, K, N, dt)
+        if need:
+            ws = _WS.get("linear_fp8", need, x.device, handle, side=side)
     _lib.check(L.moe_linear_fp8(
         x.data_ptr(), dt, xs if T > 1 else K, _p(x_scales), w.data_ptr(), w_scales.data_ptr(),
-        _p(bias), T, K, N, odt, out.data_ptr(), _p(ws), ws.numel() if ws is not None else 0,
-        handle))
+        _p(bias), T, K, N, odt, out.data_ptr(), _p(ws), 0 if ws is None else ws.numel(), handle))
     return out
 
 
@@ -515,30 +542,32 @@ def rope_freqs(rot: int, base: float = 10000.0, factor: float = 1.0, kind: str =
     return f.to(device), mscale
 
 
-def _kv_view(k_pages, v_pages, page_table, q_starts, seq_lens, dev):
-    """The C view of a paged cache and its batch."""
-    if k_pages.dim() != 4:
+def _kv_view(dtype, dim, k_pages, v_pages, page_table, q_starts, seq_lens, dev: int):
+    """The C view of a paged cache of this type and head size, and its batch."""
+    shape = k_pages.shape
+    if len(shape) != 4:
         raise ValueError("k_pages: expected [n_pages, kv_heads, page_size, head_dim], got "
-                         f"{tuple(k_pages.shape)}")
-    dt = _dt16(k_pages, "k_pages")
-    n = k_pages.numel()
-    _req(k_pages, k_pages.dtype, "k_pages", n, dev)
-    _req(v_pages, k_pages.dtype, "v_pages", n, dev)
-    if v_pages.shape != k_pages.shape:
-        raise ValueError(f"v_pages: expected {tuple(k_pages.shape)}, got {tuple(v_pages.shape)}")
+                         f"{tuple(shape)}")
+    if v_pages.shape != shape:
+        raise ValueError(f"v_pages: expected {tuple(shape)}, got {tuple(v_pages.shape)}")
+    dt = _DT16.get(dtype)
+    P, H, page, D = shape
+    n = P * H * page * D
+    _flat(k_pages, dtype, "k_pages", n, dev)
+    _flat(v_pages, dtype, "v_pages", n, dev)
     S = seq_lens.numel()
+    _flat(seq_lens, torch.int32, "seq_lens", S, dev)
+    _flat(q_starts, torch.int32, "q_starts", S + 1, dev)
     if page_table.dim() != 2 or page_table.shape[0] != S:
         raise ValueError(f"page_table: expected [{S}, pages], got {tuple(page_table.shape)}")
-    _req(seq_lens, torch.int32, "seq_lens", device=dev)
-    _req(page_table, torch.int32, "page_table", device=dev)
-    _req(q_starts, torch.int32, "q_starts", S + 1, dev)
-    P, H, page, D = k_pages.shape
+    width = page_table.shape[1]
+    _flat(page_table, torch.int32, "page_table", S * width, dev)
+    if D != dim:
+        raise ValueError(f"q of {dim} dims, pages of {D}")
     return _lib.KvView(k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
-                       q_starts.data_ptr(), seq_lens.data_ptr(), P, H, page, D, dt, S,
-                       page_table.shape[1])
+                       q_starts.data_ptr(), seq_lens.data_ptr(), P, H, page, D, dt, S, width)
 
 
-@_on_device
 def rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor,
                v_pages: torch.Tensor, page_table: torch.Tensor, q_starts: torch.Tensor,
                seq_lens: torch.Tensor, freqs: torch.Tensor, interleaved: bool = False,
@@ -561,34 +590,42 @@ def rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torch
     The batch's arrays stay on the device: an entry out of range is not followed, and
     check_device_error reports it.  Rows behind the last sequence are left as they
     were."""
-    dt = _dt16(q, "q")
-    if q.dim() != 3:
-        raise ValueError(f"q: expected [T, H, D], got {tuple(q.shape)}")
-    T, H, D = q.shape
-    dev = q.device
-    kv = _kv_view(k_pages, v_pages, page_table, q_starts, seq_lens, dev)
-    if kv.dtype != dt or kv.head_dim != D:
-        raise ValueError(f"q of {q.dtype} and {D} dims, pages of {k_pages.dtype} and {kv.head_dim}")
-    qs = _rows(q, "q", q.dtype, q.shape, dev)
-    ks = _rows(k, "k", q.dtype, (T, kv.kv_heads, D), dev)
-    vs = _rows(v, "v", q.dtype, (T, kv.kv_heads, D), dev)
-    _req(freqs, torch.float64, "freqs", device=dev)
-    for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-        if w is not None:
-            _req(w, q.dtype, name, D, dev)
-    side, handle = _stream_of(stream, dev)
+    _dt16(q, "q")
+    dev = q.get_device()
+    if dev != torch._C._cuda_getDevice():
+        return _elsewhere(rope_cache, dev, q, k, v, k_pages, v_pages, page_table, q_starts,
+                          seq_lens, freqs, interleaved, mscale, q_weight, k_weight, eps, out,
+                          stream)
+    shape, dtype = q.shape, q.dtype
+    if len(shape) != 3:
+        raise ValueError(f"q: expected [T, H, D], got {tuple(shape)}")
+    T, H, D = shape
+    kv = _kv_view(dtype, D, k_pages, v_pages, page_table, q_starts, seq_lens, dev)
+    qs = _rows(q, "q", dtype, shape, dev)
+    new = (T, kv.kv_heads, D)
+    ks = _rows(k, "k", dtype, new, dev)
+    vs = _rows(v, "v", dtype, new, dev)
+    half = freqs.numel()
+    _flat(freqs, torch.float64, "freqs", half, dev)
+    qw = kw = None
+    if q_weight is not None:
+        _flat(q_weight, dtype, "q_weight", D, dev)
+        qw = q_weight.data_ptr()
+    if k_weight is not None:
+        _flat(k_weight, dtype, "k_weight", D, dev)
+        kw = k_weight.data_ptr()
+    side, handle = _on(stream, dev)
     if out is None:
-        out = _empty(q.shape, q.dtype, dev, side)
+        out = _new(q, shape, dtype, side)
     else:
-        _req(out, q.dtype, "out", T * H * D, dev)
+        _flat(out, dtype, "out", T * H * D, dev)
     _lib.check(_lib.lib().moe_rope_cache(
         C.byref(kv), q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0],
-        vs[1], T, H, freqs.data_ptr(), 2 * freqs.numel(), interleaved, mscale, _p(q_weight),
-        _p(k_weight), eps, out.data_ptr(), handle))
+        vs[1], T, H, freqs.data_ptr(), 2 * half, interleaved, mscale, qw, kw, eps, out.data_ptr(),
+        handle))
     return out
 
 
-@_on_device
 def attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                page_table: torch.Tensor, q_starts: torch.Tensor, seq_lens: torch.Tensor,
                scale: float | None = None, window: int = 0, sinks: torch.Tensor | None = None,
@@ -603,29 +640,32 @@ def attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     sum.  D is 64 or 128.  A row that sees no key is zero; keys that a row does not see
     have no influence, whatever their bits.  Rows behind the last sequence are left as
     they were (in a new output: undefined)."""
-    dt = _dt16(q, "q")
-    if q.dim() != 3:
-        raise ValueError(f"q: expected [T, H, D], got {tuple(q.shape)}")
-    T, H, D = q.shape
-    dev = q.device
-    kv = _kv_view(k_pages, v_pages, page_table, q_starts, seq_lens, dev)
-    if kv.dtype != dt or kv.head_dim != D:
-        raise ValueError(f"q of {q.dtype} and {D} dims, pages of {k_pages.dtype} and {kv.head_dim}")
-    qs = _rows(q, "q", q.dtype, q.shape, dev)
+    _dt16(q, "q")
+    dev = q.get_device()
+    if dev != torch._C._cuda_getDevice():
+        return _elsewhere(attn_paged, dev, q, k_pages, v_pages, page_table, q_starts, seq_lens,
+                          scale, window, sinks, out, stream, workspace)
+    shape, dtype = q.shape, q.dtype
+    if len(shape) != 3:
+        raise ValueError(f"q: expected [T, H, D], got {tuple(shape)}")
+    T, H, D = shape
+    kv = _kv_view(dtype, D, k_pages, v_pages, page_table, q_starts, seq_lens, dev)
+    qs = _rows(q, "q", dtype, shape, dev)
     if sinks is not None:
-        _req(sinks, torch.float32, "sinks", H, dev)
-    side, handle = _stream_of(stream, dev)
+        _flat(sinks, torch.float32, "sinks", H, dev)
+    side, handle = _on(stream, dev)
     if out is None:
-        out = _empty(q.shape, q.dtype, dev, side)
+        out = _new(q, shape, dtype, side)
     else:
-        _req(out, q.dtype, "out", T * H * D, dev)
-    L = _lib.lib()
-    need = L.moe_attn_paged_workspace(C.byref(kv), T, H, window)
+        _flat(out, dtype, "out", T * H * D, dev)
+    L, view = _lib.lib(), C.byref(kv)
     ws = workspace
-    if ws is None and need:
-        ws = _WS.get("attn_paged", need, dev, handle, side=side)
+    if ws is None:
+        need = L.moe_attn_paged_workspace(view, T, H, window)
+        if need:
+            ws = _WS.get("attn_paged", need, q.device, handle, side=side)
     _lib.check(L.moe_attn_paged(
-        C.byref(kv), q.data_ptr(), qs[0] if T > 1 else 0, qs[1] if H > 1 else 0, T, H,
+        view, q.data_ptr(), qs[0] if T > 1 else 0, qs[1] if H > 1 else 0, T, H,
         D ** -0.5 if scale is None else scale, window, _p(sinks), out.data_ptr(), _p(ws),
-        ws.numel() if ws is not None else 0, handle))
+        0 if ws is None else ws.numel(), handle))
     return out
