@@ -358,7 +358,7 @@ int moe_linear_fp8(const void *x, int32_t x_dtype, int64_t x_stride, const float
 /*
  * A key/value cache in pages and the batch that uses it.  k, v: [n_pages,
  * kv_heads, page_size, head_dim] of `dtype`; page_size a power of two in [16,
- * 256].  Sequence s holds lens[s] tokens, the new ones included, token j in page
+ * 256]; a table row covers up to 2^30 positions.  Sequence s holds lens[s] tokens, the new ones included, token j in page
  * table[s, j / page_size]; its new tokens are the batch's rows starts[s] to
  * starts[s + 1], and row starts[s] + i is at position lens[s] - (starts[s + 1] -
  * starts[s]) + i.  The arrays are on the device: entries out of range (pages,

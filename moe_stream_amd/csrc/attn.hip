@@ -230,9 +230,6 @@ __device__ __forceinline__ uint64_t bit_range(int a, int b) {
   return (~0ull >> (64 - (b - a))) << a;
 }
 
-// What rows without a page read instead, a load's worth.
-__device__ const uint4 g_no_page[64] = {};
-
 // QW waves side by side on RB rows each share the tiles of keys; or KW waves take
 // every KW-th tile for the same RB rows and are joined at the end.
 //
@@ -242,7 +239,7 @@ __device__ const uint4 g_no_page[64] = {};
 // two waves of a SIMD do not (measured: a wave of products alone beside a wave of
 // multiply-adds alone takes longer than one after the other), so the pairs are made here.
 template <class T, int D, int RB, int QW, int KW, int BK>
-__global__ __launch_bounds__(64 * QW * KW, QW > 1 ? 2 : 1) void attn_kernel(AttnArgs a,
+__global__ __launch_bounds__(64 * QW * KW, QW > 4 ? 2 : QW > 1 ? 3 : 1) void attn_kernel(AttnArgs a,
                                                                           AttnPlan p) {
   static_assert(QW == 1 || KW == 1, "one of the two");
   using M = Mat<T>;
@@ -284,31 +281,38 @@ __global__ __launch_bounds__(64 * QW * KW, QW > 1 ? 2 : 1) void attn_kernel(Attn
   const int k1 = min(tl.end, k0 + per);
 
   const int32_t *table = kv.table + (int64_t)it.seq * kv.width;
-  auto entry_of = [&](int j0) {   // lane j: the page of key j0 + j, -1 past the end
-    const int j = j0 + lane;
-    return lane < BK && j < k1 ? table[j >> kv.page_shift] : -1;
+  // Lane j: the page of key j0 + j, past the end that of the last key.
+  auto entry_of = [&](int j0) {
+    return table[(uint32_t)min(j0 + lane, k1 - 1) >> kv.page_shift];
   };
   auto k_tile = [&](auto odd) { return (decltype(odd)::value ? lds_k1 : lds_k0) + wk * kTileBytes; };
   auto v_tile = [&](auto odd) { return (decltype(odd)::value ? lds_v1 : lds_v0) + wk * kTileBytes; };
-  // Lane j: where key j0 + j's row of K starts, or that of V.  Rows of one load lie in
-  // one page (pages hold 16 rows or more, and tiles start at a multiple of 32), so a load
-  // goes from its first row's address, and the lanes' places in it are the wave's own.
+  // Lane j: the address of key j0 + j's row of K; V's is as far from it as the arrays
+  // are.  A row without a page is read from page 0, and not used.  Rows of one load lie
+  // in one page (pages hold 16 rows or more, and tiles start at a multiple of 32), so a
+  // load goes from its first row's address, and the lanes' places in it are the wave's own.
+  const uint32_t page_bytes = (uint32_t)kv.heads << kv.page_shift << (D == 128 ? 8 : 7);
+  const uint64_t k_base =
+      reinterpret_cast<uint64_t>(kv.k) + ((uint64_t)(uint32_t)hk << kv.page_shift) * (2 * D);
+  const int64_t v_from_k =
+      reinterpret_cast<const char *>(kv.v) - reinterpret_cast<const char *>(kv.k);
   auto rows_of = [&](int j0, int entry) {
-    return page_row(entry, kv.n_pages, kv.heads, hk, kv.page_shift, j0 + lane, D);
-  };
-  auto start_of = [&](const uint16_t *pages, int64_t row) {
-    return reinterpret_cast<uint64_t>(row >= 0 ? pages + row
-                                               : reinterpret_cast<const uint16_t *>(g_no_page));
+    const uint32_t e = (uint32_t)entry < (uint32_t)kv.n_pages ? (uint32_t)entry : 0u;
+    const uint32_t in_page = (uint32_t)((j0 + lane) & ((1 << kv.page_shift) - 1)) * (2 * D);
+    return (uint64_t)e * page_bytes + (k_base + in_page);
   };
   const int sub = lane / kPieces, piece = lane % kPieces;
-  auto fetch = [&](bool is_v, uint64_t start, int i, char *to) __attribute__((always_inline)) {
+  auto fetch = [&](bool is_v, uint64_t rows, int i, char *to) __attribute__((always_inline)) {
     const int n = i * QW + wq, row = n * kRowsPerLoad;
     const int swz = is_v ? swz_v<D, RB>(row + sub) : swz_k<D>(row + sub);
-    const uint32_t at = sub * (2 * D) + (piece ^ swz) * 16;
-    const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)start, row);
-    const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(start >> 32), row);
-    const char *src = reinterpret_cast<const char *>(((uint64_t)hi << 32) | lo) + at;
-    __builtin_amdgcn_global_load_lds((global_void *)src, (lds_void *)(to + n * 1024), 16, 0, 0);
+    uint32_t at = sub * (2 * D) + (piece ^ swz) * 16;
+    asm("" : "+v"(at));   // (a 32-bit offset from a scalar address)
+    const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)rows, row);
+    const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(rows >> 32), row);
+    const char *src =
+        reinterpret_cast<const char *>((((uint64_t)hi << 32) | lo) + (is_v ? v_from_k : 0));
+    __builtin_amdgcn_global_load_lds((global_void *)(src + at), (lds_void *)(to + n * 1024), 16, 0,
+                                     0);
   };
 
   // this lane's row
@@ -333,7 +337,9 @@ __global__ __launch_bounds__(64 * QW * KW, QW > 1 ? 2 : 1) void attn_kernel(Attn
 
   // Keys of a tile that have a page; whether every row sees all of it; the keys that
   // this lane's row sees.
-  auto valid_of = [&](int entry) { return __ballot(entry >= 0 && entry < kv.n_pages); };
+  auto valid_of = [&](int j0, int entry) {
+    return __ballot((uint32_t)entry < (uint32_t)kv.n_pages) & bit_range(0, min(BK, k1 - j0));
+  };
   auto is_full = [&](int j0, uint64_t valid) {
     return j0 >= tl.full0 && j0 + BK <= tl.full1 &&
            (uint64_t)(valid << (64 - BK)) >> (64 - BK) == ~0ull >> (64 - BK);
@@ -356,7 +362,7 @@ __global__ __launch_bounds__(64 * QW * KW, QW > 1 ? 2 : 1) void attn_kernel(Attn
   constexpr int kVals = BK / NG;                           // scores of a tile a lane
   constexpr int kMulS = BK / RB * (D / (8 * NG));          // products of the scores
   constexpr int kMulO = kSteps * (D / RB);                 // and of the output
-  constexpr int kAheadK = 4, kAheadV = 3;                  // operands read ahead
+  constexpr int kAheadK = QW == 4 ? 3 : 4, kAheadV = 3;    // operands read ahead
   typedef Acc Scores[BK / RB];
 
   // Where a lane reads in a tile, but for the operand's number: the pieces' permutation is
@@ -515,8 +521,8 @@ __global__ __launch_bounds__(64 * QW * KW, QW > 1 ? 2 : 1) void attn_kernel(Attn
   // i + 1 and the values of tile i land; what step i - 1 read is free for the next.
   auto key_of = [&](int i) { return k0 + (wk + i * KW) * BK; };
   const int n = (max(0, k1 - k0 - wk * BK) + BK * KW - 1) / (BK * KW);
-  int e0 = n > 0 ? entry_of(key_of(0)) : -1;
-  const int e1 = n > 1 ? entry_of(key_of(1)) : -1;
+  int e0 = 0, e1 = 0;
+  if (n > 0) e0 = entry_of(key_of(0)), e1 = entry_of(key_of(1));
   load_q();
   // A workgroup barrier alone does not wait for loads that go to LDS.  (As a builtin, so
   // that the compiler knows of the wait and adds none of its own before the reads.)
@@ -529,21 +535,19 @@ __global__ __launch_bounds__(64 * QW * KW, QW > 1 ? 2 : 1) void attn_kernel(Attn
   Scores s0, s1;
   bool full = true;
   uint64_t vis = 0, valid_next = 0;
-  int64_t rows = 0;   // lane j: row j of tile i + 1
+  uint64_t rows = 0;   // of tile i + 1
   if (n > 0) {
-    rows = rows_of(key_of(0), e0);
-    const uint64_t kp = start_of(kv.k, rows), vp = start_of(kv.v, rows);
+    const uint64_t first = rows_of(key_of(0), e0);
 #pragma unroll
-    for (int k = 0; k < kLoads; ++k) fetch(false, kp, k, k_tile(No()));
+    for (int k = 0; k < kLoads; ++k) fetch(false, first, k, k_tile(No()));
     landed();
-    const uint64_t valid = valid_of(e0);
+    const uint64_t valid = valid_of(key_of(0), e0);
     rows = rows_of(key_of(1), e1);
-    const uint64_t kp1 = start_of(kv.k, rows);
-    valid_next = valid_of(e1);
-    e0 = n > 2 ? entry_of(key_of(2)) : -1;
+    valid_next = valid_of(key_of(1), e1);
+    e0 = entry_of(key_of(2));
     weigh(s0, s0, k_tile(No()), No(), Yes(), [&](int k) __attribute__((always_inline)) {
-      if (k < kLoads) fetch(true, vp, k, v_tile(No()));
-      else if (n > 1) fetch(false, kp1, k - kLoads, k_tile(Yes()));
+      if (k < kLoads) fetch(true, first, k, v_tile(No()));
+      else fetch(false, rows, k - kLoads, k_tile(Yes()));
     });
     full = is_full(key_of(0), valid);
     if (!full) hide(s0, vis = seen_of(key_of(0), valid));
@@ -555,19 +559,16 @@ __global__ __launch_bounds__(64 * QW * KW, QW > 1 ? 2 : 1) void attn_kernel(Attn
     using Other = std::bool_constant<!decltype(odd)::value>;   // tile i + 1's buffers
     landed();
     const uint64_t valid = valid_next;
-    uint64_t vp = 0, kp = 0;
-    const bool more = i + 2 < n;
-    if constexpr (kNext) {
-      vp = start_of(kv.v, rows);
+    const uint64_t rows_v = rows;
+    if constexpr (kNext) {   // (tiles past the end are some tile's again, not used)
       rows = rows_of(key_of(i + 2), e0);
-      kp = start_of(kv.k, rows);
-      valid_next = valid_of(e0);
-      e0 = i + 3 < n ? entry_of(key_of(i + 3)) : -1;
+      valid_next = valid_of(key_of(i + 2), e0);
+      e0 = entry_of(key_of(i + 3));
     }
     if (!full) scrub(v_tile(odd), vis);
     weigh(sc, sn, k_tile(Other()), Yes(), next, [&](int k) __attribute__((always_inline)) {
-      if (k < kLoads) fetch(true, vp, k, v_tile(Other()));
-      else if (more) fetch(false, kp, k - kLoads, k_tile(odd));
+      if (k < kLoads) fetch(true, rows_v, k, v_tile(Other()));
+      else fetch(false, rows, k - kLoads, k_tile(odd));
     });
     bool full_next = true;
     uint64_t vis_next = 0;
@@ -591,6 +592,7 @@ __global__ __launch_bounds__(64 * QW * KW, QW > 1 ? 2 : 1) void attn_kernel(Attn
   } else if (i < n) {
     step(i, s0, s1, No(), No());
   }
+  __builtin_amdgcn_s_waitcnt(loads_left(0));   // (LDS is used for something else, or given back)
   l = over_groups<RB>(l, [](float u, float v) { return u + v; });
 
   if (KW > 1) {   // the waves' keys joined on wave 0, in order
@@ -740,26 +742,29 @@ bool attn_supported(int dim, int heads, int kv_heads) {
 
 namespace {
 
-// Rows of a tile: 256 (8 waves on the same keys) where a sequence brings that many
-// rows a key head on average, otherwise 32 or 16 (waves on keys of their own).
+// Rows of a tile: 256 (128 for heads of 64) on waves that share their keys, where a
+// sequence brings more than 96 rows a key head on average, otherwise 32 or 16 on waves
+// with keys of their own.
 struct AttnShape {
   int rows;
   AttnPlan plan;
   int tiles;
   bool cut;   // whether a sequence may come in parts
 };
+constexpr int kWaves64 = 4, kWaves128 = 8;   // of 32 rows
 AttnShape attn_shape(const KvArgs &kv, int heads, int window) {
   AttnShape s;
   const int group = heads / kv.heads;
   const int64_t mean = ((int64_t)kv.total * group + kv.n_seqs - 1) / kv.n_seqs;
-  s.rows = mean > 96 ? 256 : mean > 16 ? 32 : 16;
+  const bool wide = mean > 96;
+  s.rows = wide ? 32 * (kv.dim == 64 ? kWaves64 : kWaves128) : mean > 16 ? 32 : 16;
   s.plan.hpt = std::min(group, s.rows);
   s.plan.hchunks = (group + s.plan.hpt - 1) / s.plan.hpt;
   s.plan.tpt = s.rows / s.plan.hpt;
   // a tile holds a token at least
   s.tiles = (int)std::min<int64_t>(kv.total, (int64_t)kv.total / s.plan.tpt + kv.n_seqs);
-  s.plan.target = s.rows == 256 ? 512 : 1024;
-  s.plan.least = s.rows == 256 ? 512 : 256;
+  s.plan.target = s.rows == 256 ? 512 : s.rows == 32 ? 1024 : 768;
+  s.plan.least = wide ? 512 : 256;
   SeqSpan longest = {};
   longest.len = kv.width << kv.page_shift;
   s.cut = span_keys(longest, window, s.plan.tpt) > s.plan.least;
@@ -804,7 +809,7 @@ static void attn_go(const AttnArgs &a, void *ws, hipStream_t s) {
   sh.plan.po = static_cast<float *>(ws);
   sh.plan.pml = reinterpret_cast<float2 *>(sh.plan.po + attn_part_rows(a.kv, sh) * D);
   constexpr int KW = D == 128 ? 1 : 2;
-  if (sh.rows == 256) attn_run<T, D, 32, 8, 1, 64>(a, sh, s);
+  if (sh.rows > 32) attn_run<T, D, 32, D == 64 ? kWaves64 : kWaves128, 1, 64>(a, sh, s);
   else if (sh.rows == 32) attn_run<T, D, 32, 1, KW, 32>(a, sh, s);
   else attn_run<T, D, 16, 1, KW, 32>(a, sh, s);
 }

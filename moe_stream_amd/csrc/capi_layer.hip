@@ -19,8 +19,8 @@ int make_kv_args(const moe_kv_view *v, int32_t T, moe::KvArgs *kv) {
   if ((1 << shift) != v->page_size)
     return fail(MOE_ERR_INVALID, "page_size=%d must be a power of two in [16, 256]",
                 v->page_size);
-  if ((int64_t)v->table_width * v->page_size > INT32_MAX)
-    return fail(MOE_ERR_INVALID, "table_width=%d pages of %d pass 2^31 positions",
+  if ((int64_t)v->table_width * v->page_size > (1 << 30))
+    return fail(MOE_ERR_INVALID, "table_width=%d pages of %d pass 2^30 positions",
                 v->table_width, v->page_size);
   if (v->head_dim <= 0 || v->head_dim % 2 || v->head_dim > moe::kRopeMaxDim)
     return fail(MOE_ERR_INVALID, "head_dim=%d must be even, in [2, %d]", v->head_dim,

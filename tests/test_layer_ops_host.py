@@ -90,7 +90,7 @@ BAD_VIEWS = [(dict(k=None), "NULL"), (dict(lens=None), "NULL"), (dict(dtype=2), 
              (dict(page_size=8), "page_size=8"), (dict(page_size=48), "page_size=48"),
              (dict(page_size=512), "page_size=512"), (dict(head_dim=63), "head_dim=63"),
              (dict(head_dim=514), "head_dim=514"),
-             (dict(table_width=1 << 24, page_size=256), "2^31")]
+             (dict(table_width=1 << 23, page_size=256), "2^30")]
 
 
 @pytest.mark.parametrize("bad,text", BAD_VIEWS)
