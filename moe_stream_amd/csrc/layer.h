@@ -39,33 +39,50 @@ struct F16 {
   }
 };
 
-// Eight elements from p, of which the first n (1..8) exist; the others are zero.
-template <class T>
-__device__ __forceinline__ void load8(const uint16_t *p, int n, float v[8]) {
+// Eight elements from p, of which the first n exist (n < 1: none); the others are zero.
+__device__ __forceinline__ u32x4_t bits8(const uint16_t *p, int n) {
+  u32x4_t w = {0, 0, 0, 0};
   if (n >= 8) {
-    const u32x4_t w = *reinterpret_cast<const u32x4_any *>(p);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[2 * i] = T::load(w[i] & 0xffffu);
-      v[2 * i + 1] = T::load(w[i] >> 16);
-    }
+    w = *reinterpret_cast<const u32x4_any *>(p);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < n ? T::load(p[i]) : 0.f;
+    for (int i = 0; i < 8; ++i)
+      if (i < n) w[i / 2] |= (uint32_t)p[i] << (16 * (i & 1));
   }
+  return w;
 }
-template <class T>
-__device__ __forceinline__ void store8(uint16_t *p, int n, const float v[8]) {
+// The first n of eight elements to p.
+__device__ __forceinline__ void put8(uint16_t *p, int n, u32x4_t w) {
   if (n >= 8) {
-    u32x4_t w;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = T::store(v[2 * i]) | (T::store(v[2 * i + 1]) << 16);
     *reinterpret_cast<u32x4_any *>(p) = w;
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (i < n) p[i] = (uint16_t)T::store(v[i]);
+      if (i < n) p[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
   }
+}
+template <class T>
+__device__ __forceinline__ void widen8(u32x4_t w, float v[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = T::load(w[i] & 0xffffu);
+    v[2 * i + 1] = T::load(w[i] >> 16);
+  }
+}
+template <class T>
+__device__ __forceinline__ u32x4_t narrow8(const float v[8]) {
+  u32x4_t w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = T::store(v[2 * i]) | (T::store(v[2 * i + 1]) << 16);
+  return w;
+}
+template <class T>
+__device__ __forceinline__ void load8(const uint16_t *p, int n, float v[8]) {
+  widen8<T>(bits8(p, n), v);
+}
+template <class T>
+__device__ __forceinline__ void store8(uint16_t *p, int n, const float v[8]) {
+  put8(p, n, narrow8<T>(v));
 }
 
 // --- e4m3 with a scale per 128 values ----------------------------------------

@@ -359,25 +359,40 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void linear_tile_kernel(LinearArgs
   }
 }
 
-constexpr int kThinRows = 64;   // up to this many rows of x the thin kernel runs
-constexpr int kFusedRows = 16;  // and up to this many it takes x in 16 bits
+// A tile takes the blocks of 128 columns one after another, some 0.5 us each, whatever its
+// rows; the thin kernel's waves share them, and its time goes with outputs and sets of 16
+// rows.  Behind 16 rows it runs while sets times outputs stay below this (thin against tile
+// at 2048 x 5120 weights: 20 rows 8.7 us and 10.6, 32: 10.0 and 10.6, 40: 11.7 and 10.9, 64:
+// 15.9 and 11.6; 4096 x 2880, 37 rows: 9.9 and 17; 4096 x 16384, 20 rows: 28 and 19).
+constexpr int kThinRows = 64;
+constexpr int kThinWork = 12288;
+constexpr int kFusedRows = 16;  // up to this many rows it takes x in 16 bits
 
 bool linear_takes_16(int T) { return T <= kFusedRows; }
 
+static bool is_thin(int T, int N) {
+  return T <= 16 || (T <= kThinRows && (int64_t)((T + 15) / 16) * N <= kThinWork);
+}
+
+// Four sets of 16 outputs a workgroup read x and its scales once for them (one row, 2048
+// columns: 16384 outputs 11.7 us against 13.4 with one set, 32768 19.4 against 22.7); below
+// a thousand sets the workgroups are too few for that (5120 outputs 8.7 against 7.5).
 template <class T, class XT, int TT>
 static void thin_go(const LinearArgs &a, hipStream_t s) {
-  const int n_tiles = (a.N + 15) / 16;
-  if (n_tiles >= 2048)
-    hipLaunchKernelGGL((linear_thin_kernel<T, XT, TT, 4>), dim3((n_tiles + 3) / 4),
-                       dim3(64 * kThinWaves), 0, s, a);
-  else
-    hipLaunchKernelGGL((linear_thin_kernel<T, XT, TT, 1>), dim3(n_tiles), dim3(64 * kThinWaves),
-                       0, s, a);
+  const int sets = (a.N + 15) / 16;
+  const dim3 b(64 * kThinWaves);
+  if constexpr (TT == 1) {
+    if (sets >= 1024) {
+      hipLaunchKernelGGL((linear_thin_kernel<T, XT, 1, 4>), dim3((sets + 3) / 4), b, 0, s, a);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((linear_thin_kernel<T, XT, TT, 1>), dim3(sets), b, 0, s, a);
 }
 
 template <class T>
 static void linear_go(const LinearArgs &a, int x_dtype, hipStream_t s) {
-  if (a.T <= kThinRows) {
+  if (is_thin(a.T, a.N)) {
     if (x_dtype == MOE_DTYPE_BF16) thin_go<T, Bf16, 1>(a, s);
     else if (x_dtype == MOE_DTYPE_F16) thin_go<T, F16, 1>(a, s);
     else if (a.T <= 16) thin_go<T, uint8_t, 1>(a, s);
@@ -386,18 +401,24 @@ static void linear_go(const LinearArgs &a, int x_dtype, hipStream_t s) {
     else thin_go<T, uint8_t, 4>(a, s);
     return;
   }
-  auto tiles = [&](int rows, int *t_tiles) {
-    *t_tiles = (a.T + rows - 1) / rows;
-    return *t_tiles * ((a.N + rows - 1) / rows);
+  // The larger tile reads less per product; the smaller one spreads over more CUs.  A CU
+  // has two of either of the smaller ones at once, so each runs while its tiles fit that
+  // (4096 x 4096 weights, 512 rows: 25.7 us with 64, 30.8 with 128; 768: 37.9 and 30.8; 2048:
+  // 51.2 with 128, 62.7 with 256; 2304: 76.9 and 60.4; 8192 rows of 8192 outputs: 430 and 284).
+  // Nor is a tile higher than the rows need.
+  auto tiles = [&](int rows) {
+    return (int64_t)((a.T + rows - 1) / rows) * ((a.N + rows - 1) / rows);
   };
-  int tt;
-  if (const int n = tiles(256, &tt); n >= 256)
-    hipLaunchKernelGGL((linear_tile_kernel<T, 4, 8, 4, 2>), dim3(n), dim3(512), 0, s, a, tt);
-  else if (const int n = tiles(128, &tt); n >= 256)
-    hipLaunchKernelGGL((linear_tile_kernel<T, 4, 4, 2, 2>), dim3(n), dim3(256), 0, s, a, tt);
+  constexpr int kAtOnce = 2 * 256;
+  if (a.T <= 64 || tiles(64) <= kAtOnce)
+    hipLaunchKernelGGL((linear_tile_kernel<T, 2, 2, 2, 2>), dim3(tiles(64)), dim3(256), 0, s, a,
+                       (a.T + 63) / 64);
+  else if (a.T <= 128 || tiles(128) <= kAtOnce)
+    hipLaunchKernelGGL((linear_tile_kernel<T, 4, 4, 2, 2>), dim3(tiles(128)), dim3(256), 0, s, a,
+                       (a.T + 127) / 128);
   else
-    hipLaunchKernelGGL((linear_tile_kernel<T, 2, 2, 2, 2>), dim3(tiles(64, &tt)), dim3(256), 0, s,
-                       a, tt);
+    hipLaunchKernelGGL((linear_tile_kernel<T, 4, 8, 4, 2>), dim3(tiles(256)), dim3(512), 0, s, a,
+                       (a.T + 255) / 256);
 }
 
 void launch_linear(const LinearArgs &a, int x_dtype, int out_dtype, hipStream_t s) {

@@ -50,7 +50,8 @@ __global__ __launch_bounds__(256) void norm_kernel(NormArgs a) {
   if (WPR > 1) {
     if ((threadIdx.x & 63) == 0) part[wave] = ss;
     __syncthreads();
-    ss = (part[0] + part[1]) + (part[2] + part[3]);
+    ss = WPR == 4 ? (part[0] + part[1]) + (part[2] + part[3])
+                  : part[wave & ~1] + part[wave | 1];
   }
   if (!live) return;
   const float inv = 1.f / sqrtf(ss / (float)a.D + a.eps);
@@ -85,13 +86,18 @@ static void norm_go(const NormArgs &a, hipStream_t s) {
 
 template <class T>
 static void norm_type(const NormArgs &a, hipStream_t s) {
-  if (a.T >= 1024 && a.D <= 4096) {
+  // Many rows of up to 4096 columns: one or two waves a row, so that a workgroup has more
+  // rows under way.  8192 rows of 2880: 35.5 us with two waves a row (5.3 TB/s), 37.8 with
+  // one, 37.0 with four; of 1024: 11.8 with one, 14.0 with four.  At 2048 rows the two are
+  // even (10.0 us at 2880 columns); at 1024, 7.9 against four waves' 7.2, and one row takes
+  // a third of the steps with four.
+  if (a.T >= 2048 && a.D <= 4096) {
     const int nit = (a.D + 511) / 512;
     if (nit <= 1) norm_go<T, 1, 1>(a, s);
     else if (nit <= 2) norm_go<T, 1, 2>(a, s);
-    else if (nit <= 4) norm_go<T, 1, 4>(a, s);
-    else if (nit <= 6) norm_go<T, 1, 6>(a, s);
-    else norm_go<T, 1, 8>(a, s);
+    else if (nit <= 4) norm_go<T, 2, 2>(a, s);
+    else if (nit <= 6) norm_go<T, 2, 3>(a, s);
+    else norm_go<T, 2, 4>(a, s);
     return;
   }
   const int nit = (a.D + 2047) / 2048;
@@ -148,6 +154,9 @@ void launch_to_fp8(const uint16_t *x, int64_t x_stride, int dtype, int T, int K,
 // is outside the table, the pages or the batch is left out and flagged.
 // ---------------------------------------------------------------------------
 constexpr int kRopeMaxDim = 512;
+struct Pieces {
+  u32x4_t a, b;   // a lane's two runs of a head's row
+};
 
 template <class T, int TOK, bool INTER>
 __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a, int lph_log2) {
@@ -156,33 +165,7 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a, int lph_log2) {
   const KvArgs &kv = a.kv;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int t0 = blockIdx.x * TOK;
-  if (wave < TOK) {
-    const int t = t0 + wave;
-    const int s = t < kv.total ? find_seq(kv, t, lane) : -1;
-    if (lane == 0) {
-      int pos = 0, entry = -1;
-      if (s >= 0) {
-        const SeqSpan sp = kv_span(kv, s);
-        pos = sp.base + (t - sp.first);
-        if (pos >= 0) entry = kv.table[(int64_t)s * kv.width + (pos >> kv.page_shift)];
-        if (!sp.ok || entry < 0 || entry >= kv.n_pages) flag_error_bits(kErrBadBatch);
-      }
-      here_s[wave] = s >= 0;
-      pos_s[wave] = pos;
-      entry_s[wave] = entry;
-    }
-  }
-  __syncthreads();
   const int half = a.rot / 2;
-  for (int i = threadIdx.x; i < TOK * half; i += 256) {
-    const int k = i / half, p = i % half;
-    double turns = (double)pos_s[k] * (a.freqs[p] * 0.15915494309189533577);
-    turns -= rint(turns);
-    float sn, cs;
-    sincospif(2.f * (float)turns, &sn, &cs);
-    turn[k][p] = make_float2(cs * a.mscale, sn * a.mscale);
-  }
-  __syncthreads();
   const int lph = 1 << lph_log2;              // lanes a head
   const int u = threadIdx.x & (lph - 1);
   const int groups = 256 >> lph_log2;
@@ -204,34 +187,70 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a, int lph_log2) {
   }
   na = max(0, min(na, 8));
   nb = max(0, min(nb, 8));
-  for (int item = threadIdx.x >> lph_log2; item < TOK * nh; item += groups) {
+  // Head h of token k: the query's heads, then the keys', then the values'.  Its row is
+  // read two heads ahead, the first ones before the token's place is known.
+  const int items = TOK * nh;
+  auto fetch = [&](int item) __attribute__((always_inline)) {
+    const int k = min(item, items - 1) / nh, h = min(item, items - 1) % nh;
+    const int64_t t = min(t0 + k, kv.total - 1);
+    const int hk = h - a.heads, hv = hk - kv.heads;
+    const uint16_t *src = hk < 0   ? a.q + t * a.q_st + h * a.q_sh
+                          : hv < 0 ? a.k + t * a.k_st + hk * a.k_sh
+                                   : a.v + t * a.v_st + hv * a.v_sh;
+    Pieces p;
+    p.a = bits8(src + oa, na);
+    p.b = bits8(src + ob, nb);
+    return p;
+  };
+  const int first = threadIdx.x >> lph_log2;
+  Pieces now = fetch(first), next = fetch(first + groups);
+  if (wave < TOK) {
+    const int t = t0 + wave;
+    const int s = t < kv.total ? find_seq(kv, t, lane) : -1;
+    if (lane == 0) {
+      int pos = 0, entry = -1;
+      if (s >= 0) {
+        const SeqSpan sp = kv_span(kv, s);
+        pos = sp.base + (t - sp.first);
+        if (pos >= 0) entry = kv.table[(int64_t)s * kv.width + (pos >> kv.page_shift)];
+        if (!sp.ok || entry < 0 || entry >= kv.n_pages) flag_error_bits(kErrBadBatch);
+      }
+      here_s[wave] = s >= 0;
+      pos_s[wave] = pos;
+      entry_s[wave] = entry;
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < TOK * half; i += 256) {
+    const int k = i / half, p = i % half;
+    double turns = (double)pos_s[k] * (a.freqs[p] * 0.15915494309189533577);
+    turns -= rint(turns);
+    float sn, cs;
+    sincospif(2.f * (float)turns, &sn, &cs);
+    turn[k][p] = make_float2(cs * a.mscale, sn * a.mscale);
+  }
+  __syncthreads();
+  for (int item = first; item < items; item += groups) {
+    const Pieces in = now;
+    now = next;
+    if (item + 2 * groups < items) next = fetch(item + 2 * groups);
     const int k = item / nh, h = item % nh, t = t0 + k;
     if (!here_s[k]) continue;
-    if (h >= a.heads + kv.heads) {            // a value head: as it is
-      const int hv = h - a.heads - kv.heads;
-      const int64_t at =
-          page_row(entry_s[k], kv.n_pages, kv.heads, hv, kv.page_shift, pos_s[k], D);
-      if (at < 0) continue;
-      const uint16_t *src = a.v + t * a.v_st + hv * a.v_sh;
-      for (int e = 8 * u; e < D; e += 8 * lph) {
-        if (e + 8 <= D)
-          *reinterpret_cast<u32x4_any *>(kv.v + at + e) =
-              *reinterpret_cast<const u32x4_any *>(src + e);
-        else
-          for (int i = e; i < D; ++i) kv.v[at + i] = src[i];
-      }
+    const int hk = h - a.heads, hv = hk - kv.heads;
+    uint16_t *dst = hk < 0 ? a.out : hv < 0 ? kv.k : kv.v;
+    int64_t at = ((int64_t)t * a.heads + h) * D;
+    if (hk >= 0)
+      at = page_row(entry_s[k], kv.n_pages, kv.heads, hv < 0 ? hk : hv, kv.page_shift, pos_s[k], D);
+    if (at < 0) continue;
+    if (hv >= 0) {                            // a value head: as it is
+      put8(dst + at + oa, na, in.a);
+      put8(dst + at + ob, nb, in.b);
       continue;
     }
-    const bool is_q = h < a.heads;
-    const int hk = h - a.heads;
-    const uint16_t *src = is_q ? a.q + t * a.q_st + h * a.q_sh : a.k + t * a.k_st + hk * a.k_sh;
-    int64_t at = ((int64_t)t * a.heads + h) * D;
-    if (!is_q) at = page_row(entry_s[k], kv.n_pages, kv.heads, hk, kv.page_shift, pos_s[k], D);
-    uint16_t *dst = is_q ? a.out : kv.k;
     float va[8], vb[8];
-    load8<T>(src + oa, na, va);
-    load8<T>(src + ob, nb, vb);
-    const uint16_t *w = is_q ? a.qw : a.kw;
+    widen8<T>(in.a, va);
+    widen8<T>(in.b, vb);
+    const uint16_t *w = hk < 0 ? a.qw : a.kw;
     if (w != nullptr) {
       float ss = 0.f;
 #pragma unroll
@@ -268,9 +287,8 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a, int lph_log2) {
         }
       }
     }
-    if (at < 0) continue;
-    if (na > 0) store8<T>(dst + at + oa, na, va);
-    if (nb > 0) store8<T>(dst + at + ob, nb, vb);
+    put8(dst + at + oa, na, narrow8<T>(va));
+    put8(dst + at + ob, nb, narrow8<T>(vb));
   }
 }
 
@@ -279,7 +297,10 @@ static void rope_go(const RopeArgs &a, hipStream_t s) {
   const int units = (a.rot / 2 + 7) / 8 + (a.kv.dim - a.rot + 15) / 16;
   int lg = 0;
   while ((1 << lg) < units) ++lg;
-  if (a.kv.total >= 1024)
+  // Four tokens a workgroup share its look-up from 2048 tokens on (4096 tokens of 80 heads
+  // of 64: 17.1 us against 20.2 with one; 2048: 12.3 against 13.3).  Fewer tokens need the
+  // workgroups (1024 tokens: 10.4 us against 8.4; 61: 10.4 against 6.3).
+  if (a.kv.total >= 2048)
     hipLaunchKernelGGL((rope_kernel<T, 4, INTER>), dim3((a.kv.total + 3) / 4), dim3(256), 0, s, a,
                        lg);
   else
