@@ -68,6 +68,9 @@ def test_linear_refusals():
     _refused(call(w=FAKE + 8), "aligned")
     _refused(call(x=FAKE + 8), "aligned")
     _refused(call(st=264), "aligned")
+    # a tile's rows lie within 32-bit offsets, a product in one launch
+    _refused(call(st=(1 << 23) + 16), "2^23")
+    _refused(call(T=(1 << 24) - 1, K=16, N=1 << 22), "one launch")
     # 16-bit rows beyond the few that are quantised on the way need room for their codes
     _refused(call(xd=0, xs=None, T=50, work=None), "workspace")
     _refused(call(xd=0, xs=None, T=50, work=FAKE + 16), "workspace")
