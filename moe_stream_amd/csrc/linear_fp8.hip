@@ -186,25 +186,13 @@ typedef __attribute__((address_space(3))) void lds_void;
 typedef const __attribute__((address_space(1))) void global_void;
 
 template <class T, int RT, int RN, int WT, int WN>
-__global__ __launch_bounds__(64 * WT * WN, 2) void linear_tile_kernel(LinearArgs a, int t_tiles) {
+__device__ __forceinline__ void linear_tile(const LinearArgs &a, int t0, int n0, char *lds_x0,
+                                            char *lds_x1, char *lds_w0, char *lds_w1) {
   constexpr int W = WT * WN;
   constexpr int kT = 16 * RT * WT, kN = 16 * RN * WN;
   constexpr int kLoadsX = kT / 8 / W, kLoadsW = kN / 8 / W;   // a wave's, 8 rows each
-  // (an array of its own for each tile: loads to one are under way while another is
-  // read, which the compiler waits for unless it tells them apart)
-  __shared__ __align__(1024) char lds_x0[kT * kFp8Block], lds_x1[kT * kFp8Block];
-  __shared__ __align__(1024) char lds_w0[kN * kFp8Block], lds_w1[kN * kFp8Block];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // Neighbouring workgroups go to the 8 dies in turn: each die takes a run of tiles, and
-  // within bands of 8 row tiles all of an output tile before the next, so that the tiles
-  // a die has at once read few rows of x and of w.
-  const int total = gridDim.x, each = total / 8, more = total % 8;
-  const int die = blockIdx.x % 8;
-  const int tile = die * each + min(die, more) + blockIdx.x / 8;
-  const int n_tiles = total / t_tiles, band = tile / (8 * n_tiles), in = tile % (8 * n_tiles);
-  const int wide = min(8, t_tiles - band * 8);
-  const int t0 = (band * 8 + in % wide) * kT, n0 = (in / wide) * kN;
   const int blocks = (a.K + kFp8Block - 1) / kFp8Block;
   const int last = a.K / 16 - 1;               // the last piece of a row
 
@@ -365,6 +353,40 @@ __global__ __launch_bounds__(64 * WT * WN, 2) void linear_tile_kernel(LinearArgs
   }
 }
 
+// One workgroup a tile.  kQuarters: tiles from `whole` on are cut into four, a workgroup
+// each, which the same waves take.
+template <class T, int RT, int RN, int WT, int WN, bool kQuarters>
+__global__ __launch_bounds__(64 * WT * WN, 2) void linear_tile_kernel(LinearArgs a, int t_tiles,
+                                                                      int tiles, int whole) {
+  constexpr int kT = 16 * RT * WT, kN = 16 * RN * WN;
+  // (an array of its own for each tile: loads to one are under way while another is
+  // read, which the compiler waits for unless it tells them apart)
+  __shared__ __align__(1024) char lds_x0[kT * kFp8Block], lds_x1[kT * kFp8Block];
+  __shared__ __align__(1024) char lds_w0[kN * kFp8Block], lds_w1[kN * kFp8Block];
+  // Neighbouring workgroups go to the 8 dies in turn: each die takes a run of tiles, and
+  // within bands of 8 row tiles all of an output tile before the next, so that the tiles
+  // a die has at once read few rows of x and of w.
+  const bool quarter = kQuarters && (int)blockIdx.x >= whole;
+  const int i = quarter ? blockIdx.x - whole : blockIdx.x;
+  const int total = quarter ? gridDim.x - whole : whole, each = total / 8, more = total % 8;
+  const int die = i % 8;
+  const int at = die * each + min(die, more) + i / 8;
+  const int tile = quarter ? whole + at / 4 : at;
+  const int n_tiles = tiles / t_tiles, band = tile / (8 * n_tiles), in = tile % (8 * n_tiles);
+  const int wide = min(8, t_tiles - band * 8);
+  int t0 = (band * 8 + in % wide) * kT, n0 = (in / wide) * kN;
+  if constexpr (kQuarters) {
+    if (quarter) {
+      t0 += at % 4 / 2 * (kT / 2);
+      n0 += at % 2 * (kN / 2);
+      if (t0 < a.T && n0 < a.N)
+        linear_tile<T, RT / 2, RN / 2, WT, WN>(a, t0, n0, lds_x0, lds_x1, lds_w0, lds_w1);
+      return;
+    }
+  }
+  linear_tile<T, RT, RN, WT, WN>(a, t0, n0, lds_x0, lds_x1, lds_w0, lds_w1);
+}
+
 // A tile takes the blocks of 128 columns one after another, some 0.5 us each, whatever its
 // rows; the thin kernel's waves share them, and its time goes with outputs and sets of 16
 // rows.  Behind 16 rows it runs while sets times outputs stay below this (thin against tile
@@ -415,16 +437,24 @@ static void linear_go(const LinearArgs &a, int x_dtype, hipStream_t s) {
   auto tiles = [&](int rows) {
     return (int64_t)((a.T + rows - 1) / rows) * ((a.N + rows - 1) / rows);
   };
-  constexpr int kAtOnce = 2 * 256;
-  if (a.T <= 64 || tiles(64) <= kAtOnce)
-    hipLaunchKernelGGL((linear_tile_kernel<T, 2, 2, 2, 2>), dim3(tiles(64)), dim3(256), 0, s, a,
-                       (a.T + 63) / 64);
-  else if (a.T <= 128 || tiles(128) <= kAtOnce)
-    hipLaunchKernelGGL((linear_tile_kernel<T, 4, 4, 2, 2>), dim3(tiles(128)), dim3(256), 0, s, a,
-                       (a.T + 127) / 128);
-  else
-    hipLaunchKernelGGL((linear_tile_kernel<T, 4, 8, 4, 2>), dim3(tiles(256)), dim3(512), 0, s, a,
-                       (a.T + 255) / 256);
+  constexpr int kCus = 256;
+  if (a.T <= 64 || tiles(64) <= 2 * kCus) {
+    const int n = (int)tiles(64);
+    hipLaunchKernelGGL((linear_tile_kernel<T, 2, 2, 2, 2, false>), dim3(n), dim3(256), 0, s, a,
+                       (a.T + 63) / 64, n, n);
+  } else if (a.T <= 128 || tiles(128) <= 2 * kCus) {
+    const int n = (int)tiles(128);
+    hipLaunchKernelGGL((linear_tile_kernel<T, 4, 4, 2, 2, false>), dim3(n), dim3(256), 0, s, a,
+                       (a.T + 127) / 128, n, n);
+  } else {
+    // A last round in which a quarter of the CUs or fewer would have a tile is spread over
+    // all of them (4096 x 2048 x 5120, 320 tiles: 54.6 us against 66.4; 4352 x 4096 x 4096,
+    // 272: 94.7 against 125.1).
+    const int n = (int)tiles(256), rest = n % kCus;
+    const int whole = n > kCus && rest * 4 <= kCus ? n - rest : n;
+    hipLaunchKernelGGL((linear_tile_kernel<T, 4, 8, 4, 2, true>), dim3(whole + (n - whole) * 4),
+                       dim3(512), 0, s, a, (a.T + 255) / 256, n, whole);
+  }
 }
 
 void launch_linear(const LinearArgs &a, int x_dtype, int out_dtype, hipStream_t s) {

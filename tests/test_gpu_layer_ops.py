@@ -137,7 +137,9 @@ LINEAR = [(1, 2048, 5120), (1, 16, 1), (2, 144, 130), (7, 2880, 257), (16, 4096,
           (2049, 256, 260), (515, 2048, 5120),
           # either side of where the row tiles, and the larger ones, take over
           (20, 272, 6144), (20, 272, 6160), (40, 144, 4000), (40, 144, 4200), (64, 144, 3000),
-          (64, 400, 3100), (5, 144, 16390), (16, 272, 16368), (2049, 256, 4200), (4100, 144, 2200)]
+          (64, 400, 3100), (5, 144, 16390), (16, 272, 16368), (2049, 256, 4200), (4100, 144, 2200),
+          # a last round of whole tiles cut into quarters, some of them past the end
+          (4200, 144, 4000), (4100, 272, 4100)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
