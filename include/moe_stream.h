@@ -345,7 +345,8 @@ int moe_add_rms_norm(const void *x, int64_t x_stride, const void *residual,
  * 16 bits, which the call first turns into codes and scales as moe_add_rms_norm
  * does (x_scales NULL).  w: e4m3 [N, K], w_scales [ceil(N / 128),
  * ceil(K / 128)]; bias and y [T, N] of out_dtype (16 bits).  K a multiple of 16;
- * x and w (and x's row stride) 16-byte aligned; x_stride in elements.
+ * x and w (and x's row stride) 16-byte aligned; x_stride in elements, that of 8
+ * bits up to 2^23.  T K / 128 below 2^28, T N / 65536 below 2^23.
  * workspace: at least moe_linear_fp8_workspace() bytes, 256-byte aligned; it
  * needs no zeroing.
  */
@@ -358,10 +359,10 @@ int moe_linear_fp8(const void *x, int32_t x_dtype, int64_t x_stride, const float
 /*
  * A key/value cache in pages and the batch that uses it.  k, v: [n_pages,
  * kv_heads, page_size, head_dim] of `dtype`; page_size a power of two in [16,
- * 256]; a table row covers up to 2^30 positions.  Sequence s holds lens[s] tokens, the new ones included, token j in page
- * table[s, j / page_size]; its new tokens are the batch's rows starts[s] to
- * starts[s + 1], and row starts[s] + i is at position lens[s] - (starts[s + 1] -
- * starts[s]) + i.  The arrays are on the device: entries out of range (pages,
+ * 256]; a table row covers up to 2^30 positions.  Sequence s holds lens[s]
+ * tokens, the new ones included, token j in page table[s, j / page_size]; its new
+ * tokens are the batch's rows starts[s] to starts[s + 1], and row starts[s] + i is
+ * at position lens[s] - (starts[s + 1] - starts[s]) + i.  The arrays are on the device: entries out of range (pages,
  * starts that descend or pass the batch's rows, lengths past the table or below
  * the new tokens) are not followed, and raise the device error that
  * moe_check_device_error reports as MOE_ERR_DEVICE.  Rows behind the last
@@ -401,12 +402,13 @@ int moe_rope_cache(const moe_kv_view *kv, const void *q, int64_t q_token, int64_
  * values already):
  *   out[t, h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q[t, h] . k_j)
  * over the keys j up to the row's own position, or the last `window` of those
- * (window > 0).  Head h reads key head h / (heads / kv_heads).  sinks [heads]
- * fp32 (NULL: none) adds exp(sinks[h]) to the sum below the line.  Keys that a
- * row does not see, and what pages hold past a sequence's length, have no
- * influence whatever their bits.  A row that sees no key is zero.  q at token
- * and head strides that are multiples of 8 elements, 16-byte aligned; out [T,
- * heads, head_dim] contiguous.  head_dim 64 or 128, up to 64 heads per key head.
+ * (window > 0), scale in [0, 1e30].  Head h reads key head h / (heads / kv_heads).
+ * sinks [heads] fp32 (NULL: none) adds exp(sinks[h]) to the sum below the line.
+ * Keys that a row does not see, and what pages hold past a sequence's length,
+ * have no influence whatever their bits.  A row that sees no key is zero.  q at
+ * token and head strides that are multiples of 8 elements, 16-byte aligned; out
+ * [T, heads, head_dim] contiguous.  head_dim 64 or 128, up to 64 heads per key
+ * head.
  * workspace: at least moe_attn_paged_workspace() bytes, 256-byte aligned; it
  * needs no zeroing.
  */

@@ -100,7 +100,8 @@ struct AttnItem {
 
 // Keys that the tiles of a sequence pass over, at most.
 MOE_HD int span_keys(const SeqSpan &sp, int window, int tpt) {
-  return window > 0 ? (int)((int64_t)window + tpt + 63 < sp.len ? (int64_t)window + tpt + 63 : sp.len) : sp.len;
+  const int64_t most = (int64_t)window + tpt + 63;
+  return window > 0 && most < sp.len ? (int)most : sp.len;
 }
 
 template <int CTRL, int ROWS>
@@ -238,9 +239,17 @@ __device__ __forceinline__ uint64_t bit_range(int a, int b) {
 // i + 1: a wave's vector instructions run beside its own matrix instruction, but those of
 // two waves of a SIMD do not (measured: a wave of products alone beside a wave of
 // multiply-adds alone takes longer than one after the other), so the pairs are made here.
+//
+// Many rows are bound by instruction issue: 4096 rows of 32/4 heads of 128 over 8192 keys
+// take 630 us, 1.09 PFLOP/s of the 1.24 that a large library product reaches, the matrix unit
+// busy 53 % of the cycles, no bank conflicts; 9 chunks of 64/8 heads of 64 127 us, 690
+// TFLOP/s, 33 % (two exponentials a product of 16 columns cost as much issue as it).  Few
+// rows are bound by the bytes of the keys: 48 tokens over 64/8 heads of 64 read 435 MB in
+// 82 us, 5.3 TB/s, what a large copy reaches, and join in 5 us; one token over 40000 keys
+// reads 82 MB in 17 us (4.9 TB/s) and joins in 6.
 template <class T, int D, int RB, int QW, int KW, int BK>
-__global__ __launch_bounds__(64 * QW * KW, QW > 4 ? 2 : QW > 1 ? 3 : 1) void attn_kernel(AttnArgs a,
-                                                                          AttnPlan p) {
+__global__ __launch_bounds__(64 * QW * KW, QW > 4 ? 2 : QW > 1 ? 3 : 1)
+void attn_kernel(AttnArgs a, AttnPlan p) {
   static_assert(QW == 1 || KW == 1, "one of the two");
   using M = Mat<T>;
   using Acc = typename Block<RB>::acc;
@@ -285,8 +294,12 @@ __global__ __launch_bounds__(64 * QW * KW, QW > 4 ? 2 : QW > 1 ? 3 : 1) void att
   auto entry_of = [&](int j0) {
     return table[(uint32_t)min(j0 + lane, k1 - 1) >> kv.page_shift];
   };
-  auto k_tile = [&](auto odd) { return (decltype(odd)::value ? lds_k1 : lds_k0) + wk * kTileBytes; };
-  auto v_tile = [&](auto odd) { return (decltype(odd)::value ? lds_v1 : lds_v0) + wk * kTileBytes; };
+  auto k_tile = [&](auto odd) {
+    return (decltype(odd)::value ? lds_k1 : lds_k0) + wk * kTileBytes;
+  };
+  auto v_tile = [&](auto odd) {
+    return (decltype(odd)::value ? lds_v1 : lds_v0) + wk * kTileBytes;
+  };
   // Lane j: the address of key j0 + j's row of K; V's is as far from it as the arrays
   // are.  A row without a page is read from page 0, and not used.  Rows of one load lie
   // in one page (pages hold 16 rows or more, and tiles start at a multiple of 32), so a
@@ -743,8 +756,19 @@ bool attn_supported(int dim, int heads, int kv_heads) {
 namespace {
 
 // Rows of a tile: 256 (128 for heads of 64) on waves that share their keys, where a
-// sequence brings more than 96 rows a key head on average, otherwise 32 or 16 on waves
-// with keys of their own.
+// sequence brings more than 64 rows a key head on average, otherwise 32 or 16 on waves
+// with keys of their own.  8 sequences of 9000 keys, 32/4 heads of 128: 16 rows each 37.8 us
+// on tiles of 16, 51 on 256; 24 rows 40.5 on 32 and 44.7 on 16; 64 rows 45.8 on 32, 54.7 on
+// 256 and 65 on 16; 80 rows 71 on 32 and 57 on 256; 192 rows 117 and 71.  64/8 heads of 64 go
+// alike (80 rows: 63.6 and 44.3 us).
+//   Heads of 64 leave registers for three waves a SIMD with tiles of 128 rows: 9 chunks of
+// 64/8 heads 127 us, with 256 rows 139; 4096 rows over 12288 keys 770 and 794.  Heads of 128
+// do not: 4096 rows of 32/4 heads over 8192 keys take 620 us with 256 rows, 637 with 128.
+//   target: items enough to even out the lengths, few enough that joining them is small
+// (48 single tokens, 64/8 heads of 64: 512 items 89 us, 640 91, 768 86, 1024 95; 8 x 8 tokens,
+// tiles of 32: 768 47.5, 1024 44.7).
+//   least: shorter parts would gain little (4 tokens over 3000 keys: 13.0 us with parts from
+// 128 keys, 15.2 from 256), and would give windows of 128 keys a second launch.
 struct AttnShape {
   int rows;
   AttnPlan plan;
@@ -756,7 +780,7 @@ AttnShape attn_shape(const KvArgs &kv, int heads, int window) {
   AttnShape s;
   const int group = heads / kv.heads;
   const int64_t mean = ((int64_t)kv.total * group + kv.n_seqs - 1) / kv.n_seqs;
-  const bool wide = mean > 96;
+  const bool wide = mean > 64;
   s.rows = wide ? 32 * (kv.dim == 64 ? kWaves64 : kWaves128) : mean > 16 ? 32 : 16;
   s.plan.hpt = std::min(group, s.rows);
   s.plan.hchunks = (group + s.plan.hpt - 1) / s.plan.hpt;

@@ -214,6 +214,8 @@ int moe_attn_paged(const moe_kv_view *kv, const void *q, int64_t q_token, int64_
                 "no attention kernel compiled for head_dim=%d with %d heads per key head",
                 kv->head_dim, heads / kv->kv_heads);
   if (window < 0) return fail(MOE_ERR_INVALID, "window=%d is negative", window);
+  if (!(scale >= 0.f && scale <= 1e30f))
+    return fail(MOE_ERR_INVALID, "scale=%g outside [0, 1e30]", scale);
   if (T == 0) return MOE_OK;
   if (!moe::attn_fits(a.kv, heads, window))
     return fail(MOE_ERR_UNSUPPORTED, "T=%d rows of %d heads pass one launch", T, heads);

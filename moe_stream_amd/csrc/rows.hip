@@ -13,7 +13,9 @@ namespace moe {
 // in registers, 8 elements a lane and step, so the row is read once; the sum of
 // squares is 32-bit throughout.  h is rounded to the row's type before the norm,
 // because that is the residual stream the next layer reads.  y is rounded once:
-// to the row's type, or to e4m3 straight from 32 bits.
+// to the row's type, or to e4m3 straight from 32 bits.  Bound by bytes: 8192 rows of
+// 2880 with residual to 8 bits move 166 MB in 32 us, 5.2 TB/s, a large copy's rate; one
+// row takes 1.9 us, little over an empty kernel.
 // ---------------------------------------------------------------------------
 template <class T, int WPR, int NIT, bool FP8>
 __global__ __launch_bounds__(256) void norm_kernel(NormArgs a) {
@@ -151,7 +153,9 @@ void launch_to_fp8(const uint16_t *x, int64_t x_stride, int dtype, int T, int K,
 // a fraction of a turn there: at position 2^20 a 32-bit product would be off by
 // 2^-4 radians.  The workgroup's tokens have their cosines and sines in LDS, once
 // for all heads.  Keys and values go straight to their page; a token whose place
-// is outside the table, the pages or the batch is left out and flagged.
+// is outside the table, the pages or the batch is left out and flagged.  Bound by
+// bytes when there are many (4096 tokens of 80 heads of 64: 84 MB in 16.8 us, 5.0
+// TB/s), by the chain of look-up, angle and rotation for few (61 tokens: 6.3 us).
 // ---------------------------------------------------------------------------
 constexpr int kRopeMaxDim = 512;
 struct Pieces {

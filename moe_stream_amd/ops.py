@@ -635,7 +635,7 @@ def attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     values already (rope_cache's arguments and batch).  Returns [T, H, D].
 
     q [T, H, D] with 16-byte aligned heads at any token and head strides; head h reads
-    key head h // (H / HK); scale defaults to D^-0.5.  window > 0: a row sees the last
+    key head h // (H / HK); scale in [0, 1e30], D^-0.5 by default.  window > 0: a row sees the last
     `window` positions up to its own.  sinks fp32 [H]: exp(sinks[h]) joins the softmax's
     sum.  D is 64 or 128.  A row that sees no key is zero; keys that a row does not see
     have no influence, whatever their bits.  Rows behind the last sequence are left as

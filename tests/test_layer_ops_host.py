@@ -109,8 +109,9 @@ def _rope(v, q=FAKE, T=3, H=8, f=FAKE, rot=64, eps=1e-6, out=FAKE):
                                      rot, 0, 1.0, None, None, eps, out, None)
 
 
-def _attn(v, q=FAKE, qt=512, qh=64, T=3, H=8, window=0, out=FAKE, work=FAKE, n=1 << 40):
-    return _lib.lib().moe_attn_paged(C.byref(v), q, qt, qh, T, H, 0.125, window, None, out, work,
+def _attn(v, q=FAKE, qt=512, qh=64, T=3, H=8, window=0, out=FAKE, work=FAKE, n=1 << 40,
+          scale=0.125):
+    return _lib.lib().moe_attn_paged(C.byref(v), q, qt, qh, T, H, scale, window, None, out, work,
                                      n, None)
 
 
@@ -137,6 +138,8 @@ def test_attn_refusals():
     _refused(_attn(v, H=130), "65 heads", _lib.MOE_ERR_UNSUPPORTED)
     _refused(_attn(_view(head_dim=80)), "head_dim=80", _lib.MOE_ERR_UNSUPPORTED)
     _refused(_attn(v, window=-1), "window=-1")
+    for scale in (-0.125, float("nan"), float("inf")):
+        _refused(_attn(v, scale=scale), "scale")
     _refused(_attn(v, q=None), "NULL")
     _refused(_attn(v, out=None), "NULL")
     _refused(_attn(v, q=FAKE + 8), "aligned")
