@@ -183,9 +183,8 @@ __global__ __launch_bounds__(64 * kThinWaves) void linear_thin_kernel(LinearArgs
 // 128 bytes span the banks) so that 16 rows' reads of a piece meet no conflict.  The
 // scales of the lane's rows are a block ahead in registers.  8192 x 4096 x 8192 takes 284
 // us, 1.94 PFLOP/s (a large library product of unscaled blocks: 2.78); 4096 x 2048 x 5120 54
-// us, 1.6.  The matrix unit is busy a quarter to a half of the cycles: the reads of the
-// operands from LDS, one for two products of 16 x 16, and the folds, four multiply-adds a
-// product, go between.
+// us, 1.6, with the matrix unit busy 30 % of the cycles: the reads of the operands from
+// LDS and the folds, four multiply-adds a product, go between.
 // ---------------------------------------------------------------------------
 typedef __attribute__((address_space(3))) void lds_void;
 typedef const __attribute__((address_space(1))) void global_void;
