@@ -444,7 +444,8 @@ def linear_fp8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor,
     output), or 16 bits, quantised the same way on the way in; w float8_e4m3fn [N, K]
     with w_scales fp32 [ceil(N / 128), ceil(K / 128)]; bias [N] of the output's type:
     `dtype` (bf16 or fp16), else out's, else x's where it has 16 bits, else bf16.
-    K is a multiple of 16.  Returns y [T, N] ([N] for x [K])."""
+    K is a multiple of 16.  workspace: uint8 on x's device, moe_linear_fp8_workspace
+    bytes, by default one of the stream's own.  Returns y [T, N] ([N] for x [K])."""
     x8 = x.dtype is torch.float8_e4m3fn
     if not x8:
         dt = _dt16(x, "x")
@@ -489,7 +490,9 @@ def linear_fp8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor,
         _flat(out, dtype, "out", T * N, dev)
     L = _lib.lib()
     ws = workspace
-    if ws is None and not x8:
+    if ws is not None:
+        _flat(ws, torch.uint8, "workspace", ws.numel(), dev)
+    elif not x8:
         need = L.moe_linear_fp8_workspace(T, K, N, dt)
         if need:
             ws = _WS.get("linear_fp8", need, x.device, handle, side=side)
@@ -639,7 +642,8 @@ def attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     `window` positions up to its own.  sinks fp32 [H]: exp(sinks[h]) joins the softmax's
     sum.  D is 64 or 128.  A row that sees no key is zero; keys that a row does not see
     have no influence, whatever their bits.  Rows behind the last sequence are left as
-    they were (in a new output: undefined)."""
+    they were (in a new output: undefined).  workspace: uint8 on q's device,
+    moe_attn_paged_workspace bytes, by default one of the stream's own."""
     _dt16(q, "q")
     dev = q.get_device()
     if dev != torch._C._cuda_getDevice():
@@ -660,7 +664,9 @@ def attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
         _flat(out, dtype, "out", T * H * D, dev)
     L, view = _lib.lib(), C.byref(kv)
     ws = workspace
-    if ws is None:
+    if ws is not None:
+        _flat(ws, torch.uint8, "workspace", ws.numel(), dev)
+    else:
         need = L.moe_attn_paged_workspace(view, T, H, window)
         if need:
             ws = _WS.get("attn_paged", need, q.device, handle, side=side)

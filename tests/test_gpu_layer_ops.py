@@ -453,6 +453,26 @@ def test_attn_over_a_long_context():
     within(ops.attn_paged(b.q, *b.pages()), ref, _attn_bound(ref, mag, BF16))
 
 
+def test_workspaces_given():
+    b = Batch([(2, 5000), (1, 90)], 8, 2, 64, 16, seed=183)
+    w, ws = _weights(130, 256, 185)
+    x = randn((70, 256), 187)
+    o, y = ops.attn_paged(b.q, *b.pages()), ops.linear_fp8(x, w, ws)
+    room = torch.full((1 << 24,), 0xff, dtype=torch.uint8, device="cuda")   # NaN bits
+    assert torch.equal(ops.attn_paged(b.q, *b.pages(), workspace=room), o)
+    assert torch.equal(ops.linear_fp8(x, w, ws, workspace=room), y)
+    for bad in (room.cpu(), room.view(torch.int8), room[::2]):
+        with pytest.raises((TypeError, ValueError)):
+            ops.attn_paged(b.q, *b.pages(), workspace=bad)
+        with pytest.raises((TypeError, ValueError)):
+            ops.linear_fp8(x, w, ws, workspace=bad)
+    for f in (lambda: ops.attn_paged(b.q, *b.pages(), workspace=room[:256]),
+              lambda: ops.linear_fp8(x, w, ws, workspace=room[:256]),
+              lambda: ops.linear_fp8(x, w, ws, workspace=room[16:])):
+        with pytest.raises(_lib.MoeError):
+            f()
+
+
 # -- entries out of range --------------------------------------------------------------
 def _reported():
     with pytest.raises(_lib.MoeError) as e:
