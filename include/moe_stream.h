@@ -405,10 +405,10 @@ int moe_rope_cache(const moe_kv_view *kv, const void *q, int64_t q_token, int64_
  * (window > 0), scale in [0, 1e30].  Head h reads key head h / (heads / kv_heads).
  * sinks [heads] fp32 (NULL: none) adds exp(sinks[h]) to the sum below the line.
  * Keys that a row does not see, and what pages hold past a sequence's length,
- * have no influence whatever their bits.  A row that sees no key is zero.  q at
- * token and head strides that are multiples of 8 elements, 16-byte aligned; out
- * [T, heads, head_dim] contiguous.  head_dim 64 or 128, up to 64 heads per key
- * head.
+ * have no influence whatever their bits.  A row that sees no key is zero (and one
+ * whose scores are all -infinity).  q at token and head strides that are
+ * multiples of 8 elements, 16-byte aligned; out [T, heads, head_dim] contiguous.
+ * head_dim 64 or 128, up to 64 heads per key head.
  * workspace: at least moe_attn_paged_workspace() bytes, 256-byte aligned; it
  * needs no zeroing.
  */

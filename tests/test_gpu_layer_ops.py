@@ -44,7 +44,11 @@ pytestmark = pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("T,D", [(1, 2048), (3, 2880), (1, 1), (5, 7), (2, 127), (4, 129),
                                  (1025, 512), (1100, 2880), (1030, 1001), (2, 4097), (3, 8192),
-                                 (2, 16384), (1024, 4096), (1027, 65)])
+                                 (2, 16384), (1024, 4096), (1027, 65),
+                                 # one and two waves a row
+                                 (2049, 65), (2051, 512), (2050, 1001), (2049, 1032), (2053, 2000),
+                                 (2049, 2051), (2048, 2880), (2050, 3100), (2049, 4096),
+                                 (2049, 4104)])
 def test_norm_16_bits(T, D, dtype):
     x, r = randn((T, D), 11, dtype, 0.7), randn((T, D), 12, dtype, 3.0)
     w = randn((D,), 13, dtype)
@@ -59,7 +63,9 @@ def test_norm_16_bits(T, D, dtype):
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("T,D", [(1, 2048), (3, 2880), (2, 5), (3, 130), (1100, 2880), (1029, 333),
-                                 (2, 6001), (1030, 4096)])
+                                 (2, 6001), (1030, 4096),
+                                 # one and two waves a row
+                                 (2049, 100), (2051, 1000), (2049, 1170), (2050, 2880), (2049, 4096)])
 def test_norm_8_bits(T, D, dtype):
     x, r, w = randn((T, D), 21, dtype), randn((T, D), 22, dtype), randn((D,), 23, dtype)
     q, s, h = ops.add_rms_norm(x, w, residual=r, fp8=True)
@@ -204,7 +210,12 @@ ROPE = [dict(seqs=[(1, 1)], H=4, HK=1, D=64, R=64, page=16),
         dict(seqs=[(3, 2 ** 20), (2, 77)], H=4, HK=4, D=128, R=64, page=256, norm=True),
         dict(seqs=[(9, 11)], H=3, HK=3, D=10, R=6, page=16, norm=True),
         dict(seqs=[(2, 33)], H=2, HK=1, D=512, R=512, page=16),
-        dict(seqs=[(4, 9)], H=2, HK=2, D=64, R=0, page=16, norm=True)]
+        dict(seqs=[(4, 9)], H=2, HK=2, D=64, R=0, page=16, norm=True),
+        # four tokens a workgroup, of several sequences
+        dict(seqs=[(700, 900), (0, 5), (1401, 1401), (1, 3), (1, 1), (2, 70)], H=8, HK=2, D=64, R=32,
+             page=32, norm=True, inter=True),
+        dict(seqs=[(2047, 2600), (3, 3)], H=6, HK=2, D=80, R=80, page=128),
+        dict(seqs=[(2, 9)] * 1030, H=3, HK=1, D=10, R=6, page=16, norm=True)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
@@ -365,6 +376,27 @@ def test_attn_rows_that_see_nothing():
         with pytest.raises(_lib.MoeError) as e:
             ops.check_device_error()
         assert e.value.code == _lib.MOE_ERR_DEVICE
+
+
+@pytest.mark.parametrize("n", [1, 90])
+def test_attn_scores_of_infinity(n):
+    """A key of -infinity weighs nothing; a row of nothing else is zero; +infinity is NaN."""
+    b = Batch([(n, 200), (n, n)], 8, 1, 64, 16, seed=189)
+    b.q.abs_().add_(0.1)
+    b.kp[b.table[0, 3].long(), :, 5] = float("-inf")         # key 53 of the first
+    b.kp[b.table[1].long()] = float("-inf")                  # all of the second
+    got = ops.attn_paged(b.q, *b.pages())
+    t = b.table[0].long()
+    for i in range(n):
+        j = torch.arange(200 - n + i + 1, device="cuda")
+        k, v = (x[t[j // 16], 0, j % 16].double() for x in (b.kp, b.vp))
+        p = torch.softmax(b.q[i].double() @ k.T / 8, -1)
+        ref, mag = p @ v, p @ v.abs()
+        within(got[i], f64(ref), f64(ref.abs() * 2.0 ** -8 + (2.0 ** -8 + 2.0 ** -14) * mag))
+    assert (got[n:] == 0).all()
+    b.kp[b.table[0, 3].long(), :, 5] = float("inf")
+    got = ops.attn_paged(b.q, *b.pages())
+    assert got[:n].isnan().all() and (got[n:] == 0).all()
 
 
 def test_attn_sink_of_minus_infinity_is_none():
