@@ -346,7 +346,7 @@ int moe_add_rms_norm(const void *x, int64_t x_stride, const void *residual,
  * does (x_scales NULL).  w: e4m3 [N, K], w_scales [ceil(N / 128),
  * ceil(K / 128)]; bias and y [T, N] of out_dtype (16 bits).  K a multiple of 16;
  * x and w (and x's row stride) 16-byte aligned; x_stride in elements, that of 8
- * bits up to 2^23.  T K / 128 below 2^28, T N / 65536 below 2^23.
+ * bits up to 2^23.  T K / 128 below 2^28, T N / 65536 below 2^22.
  * workspace: at least moe_linear_fp8_workspace() bytes, 256-byte aligned; it
  * needs no zeroing.
  */
