@@ -108,7 +108,8 @@ int moe_linear_fp8(const void *x, int32_t x_dtype, int64_t x_stride, const float
   if (T == 0) return MOE_OK;
   if ((int64_t)T * ((K + moe::kFp8Block - 1) / moe::kFp8Block) >= (1 << 28))
     return fail(MOE_ERR_INVALID, "T=%d rows of K=%d pass one launch", T, K);
-  // (tiles of 256, or their quarters, in one launch of 512 threads each; a tile's rows of x lie within 32 bits)
+  // (tiles of 256, or their quarters, in one launch of 512 threads each; a tile's rows of
+  // x lie within 32 bits)
   if ((int64_t)((T + 255) / 256) * ((N + 255) / 256) >= (1 << 22))
     return fail(MOE_ERR_INVALID, "T=%d rows of N=%d outputs pass one launch", T, N);
   if (x8 && T > 1 && x_stride > (1 << 23))
